@@ -327,6 +327,72 @@ int    vt_gemm_tn_f32b(const double* A_dev, int64_t lda, int Da, const float* B_
                        const double* rowscale_dev, int64_t N, double alpha, const double* bias_dev,
                        double* C_dev, int64_t ldc, void* ws_dev, size_t ws_bytes, void* stream);
 
+/* ---- Compact rows: microscaled 8-bit and 4-bit floating point ------------------------------------------
+ * A row of D numbers is cut into nb = ceil(D / 32) blocks of 32 columns.  A block is one scale byte s, standing for
+ * 2^(s - 127) (255: the whole block is NaN), and 32 codes: VT_MX_FP8 = E4M3 (1 sign, 4 exponent, 3 mantissa bits; 32
+ * bytes a block), VT_MX_FP4 = E2M1 (magnitudes 0 .5 1 1.5 2 3 4 6; 16 bytes a block, the even column in the low half
+ * of a byte).  The value of an element is code * 2^(s - 127), in the range of float.  Codes of the columns >= D of the
+ * last block are 0.
+ *   codes  : (N, ldc) bytes, 16-byte aligned, ldc a multiple of 16, >= nb * 32 (FP8) or nb * 16 (FP4)
+ *   scales : (N, lds) bytes, lds >= nb
+ * The reference keeps its arrays in fp64 and has no counterpart; the row operators below take the place of the same
+ * lines as their fp64 namesakes (vt_glm_link, ...) for rows that are stored this way. */
+#define VT_MX_FP4 0
+#define VT_MX_FP8 1
+#define VT_TYPE_F64  0
+#define VT_TYPE_F32  1
+#define VT_TYPE_BF16 2
+#define VT_TYPE_F16  3
+
+/* codes, scales <- X (N, D; element stride 1, row stride ldx).  Scale: the smallest power of two in 2^-127 .. 2^127
+ * with which the largest magnitude of the block still rounds to a finite code, so nothing saturates; codes: round to
+ * nearest, ties to even, from the full precision of X.  A block that holds NaN, an infinity or a magnitude that
+ * rounds past the largest float gets s = 255 and codes 0. */
+int    vt_mx_quantise(int type, const void* X_dev, int64_t ldx, int64_t N, int D, int format, void* codes_dev,
+                      int64_t ldc, void* scales_dev, int64_t lds, void* stream);
+/* out (N, D; row stride ldo) <- the values, rounded to `type` (exact for F32, F64; BF16 too but for subnormals). */
+int    vt_mx_dequantise(int format, const void* codes_dev, int64_t ldc, const void* scales_dev, int64_t lds,
+                        int64_t N, int D, int type, void* out_dev, int64_t ldo, void* stream);
+
+/* Row operators on compact rows: arguments, results and their fp64 vectors and sums as vt_glm_link / _grad / _value /
+ * _hvp / vt_gemv / vt_gemv_t2 (u2 may be NULL: vt_gemv_t).  D >= 1 without an upper limit. */
+size_t vt_mx_rows_workspace_bytes(int64_t N, int D);
+int    vt_mx_glm_link(int family, int format, const void* codes_dev, int64_t ldc, const void* scales_dev, int64_t lds,
+                      const double* theta_dev, const double* y_dev, const double* w_dev, const double* offset_dev,
+                      double scale, int64_t N, int D, double* z_dev, double* r_dev, double* d_dev, void* ws_dev,
+                      size_t ws_bytes, void* stream);
+int    vt_mx_glm_grad(int family, int format, const void* codes_dev, int64_t ldc, const void* scales_dev, int64_t lds,
+                      const double* theta_dev, const double* y_dev, const double* w_dev, const double* offset_dev,
+                      double scale, const double* prior_dev, int64_t N, int D, double* g_dev, double* r_dev,
+                      double* d_dev, void* ws_dev, size_t ws_bytes, void* stream);
+int    vt_mx_glm_value(int family, int format, const void* codes_dev, int64_t ldc, const void* scales_dev, int64_t lds,
+                       const double* theta_dev, const double* y_dev, const double* w_dev, const double* offset_dev,
+                       double scale, int64_t N, int D, double* value_dev, void* ws_dev, size_t ws_bytes, void* stream);
+int    vt_mx_glm_hvp(int format, const void* codes_dev, int64_t ldc, const void* scales_dev, int64_t lds,
+                     const double* d_dev, const double* prior_dev, double prior_scalar, const double* v_dev, int64_t N,
+                     int D, double* out_dev, void* ws_dev, size_t ws_bytes, void* stream);
+int    vt_mx_gemv(int format, const void* codes_dev, int64_t ldc, const void* scales_dev, int64_t lds,
+                  const double* v_dev, int64_t N, int D, double* out_dev, void* ws_dev, size_t ws_bytes, void* stream);
+int    vt_mx_gemv_t(int format, const void* codes_dev, int64_t ldc, const void* scales_dev, int64_t lds,
+                    const double* u1_dev, const double* u2_dev, int64_t N, int D, double* out_dev, void* ws_dev,
+                    size_t ws_bytes, void* stream);
+
+/* C (M, N) = alpha * A B^T + 1 bias^T for FP4 rows A (M, K) and B (N, K): scaled MFMA products, sums in float; C is
+ * float (VT_TYPE_F32) or rounded once to bfloat16 (VT_TYPE_BF16); bias (N,) float or NULL. */
+size_t vt_mx_gemm_nt_workspace_bytes(int64_t M, int64_t N, int K);
+int    vt_mx_gemm_nt(const void* codes_a_dev, int64_t ldca, const void* scales_a_dev, int64_t ldsa, int64_t M,
+                     const void* codes_b_dev, int64_t ldcb, const void* scales_b_dev, int64_t ldsb, int64_t N, int K,
+                     float alpha, const float* bias_dev, int out_type, void* C_dev, int64_t ldc, void* ws_dev,
+                     size_t ws_bytes, void* stream);
+/* C (Da, Db) = alpha * A^T diag(rowscale) B + 1 bias^T for compact rows A (N, Da) and B (N, Db) of type F32, BF16 or
+ * F16: the gradient of a linear layer's weights from its stored activations.  The product rowscale * B is rounded once
+ * to float; products are exact, sums and C are float; rowscale (N,) double or NULL, bias (Db,) float or NULL. */
+size_t vt_mx_gemm_tn_workspace_bytes(int64_t N, int Da, int Db);
+int    vt_mx_gemm_tn(int format, const void* codes_dev, int64_t ldc, const void* scales_dev, int64_t lds, int Da,
+                     int type, const void* B_dev, int64_t ldb, int Db, const double* rowscale_dev, int64_t N,
+                     float alpha, const float* bias_dev, float* C_dev, int64_t ldo, void* ws_dev, size_t ws_bytes,
+                     void* stream);
+
 /* ---- Synthetic inputs: counter-based generator ----------------------------------
  * Philox-4x32-10, key = seed, counter = (row, column pair, stream_id): any block of rows can be regenerated
  * independently (row shards of one global data set; host-side spot checks -- vittles_amd/synth.py implements the

@@ -9,6 +9,7 @@ from .objectives import RegisteredObjective, WeightedGLMObjective, HierGaussMFVI
 from .sparse_hessian_lib import SparseBlockHessian
 from .lr_cov_lib import LinearResponseCovariances
 from . import solver_lib
+from . import compact
 from . import optim
 from . import synth
 from . import bivariate_sensitivity_lib
@@ -26,6 +27,7 @@ __all__ = [
     "LinearResponseCovariances",
     "ParametricSensitivityTaylorExpansion",
     "solver_lib",
+    "compact",
     "optim",
     "bivariate_sensitivity_lib",
 ]

@@ -21,6 +21,7 @@ c_ptr = ctypes.c_void_p
 
 VT_OK = 0
 FAMILY = {"logistic": 0, "poisson": 1, "gaussian": 2}
+MX_FORMAT = {"mxfp4": 0, "mxfp8": 1}
 SMALL_D_MAX = 128
 
 # name -> (restype, argtypes); every symbol include/vittles_hip.h declares.
@@ -110,6 +111,27 @@ SIGNATURES = {
     "vt_gemv_f32": (c_int, [c_ptr, c_i64, c_ptr, c_i64, c_int, c_ptr, c_ptr, c_size_t, c_ptr]),
     "vt_glm_value_f32": (c_int, [c_int, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_dbl, c_i64, c_int,
                                  c_ptr, c_ptr, c_size_t, c_ptr]),
+    # compact rows: microscaled 8-bit and 4-bit storage
+    "vt_mx_quantise": (c_int, [c_int, c_ptr, c_i64, c_i64, c_int, c_int, c_ptr, c_i64, c_ptr, c_i64, c_ptr]),
+    "vt_mx_dequantise": (c_int, [c_int, c_ptr, c_i64, c_ptr, c_i64, c_i64, c_int, c_int, c_ptr, c_i64, c_ptr]),
+    "vt_mx_rows_workspace_bytes": (c_size_t, [c_i64, c_int]),
+    "vt_mx_glm_link": (c_int, [c_int, c_int, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_dbl, c_i64, c_int,
+                               c_ptr, c_ptr, c_ptr, c_ptr, c_size_t, c_ptr]),
+    "vt_mx_glm_grad": (c_int, [c_int, c_int, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_dbl, c_ptr, c_i64,
+                               c_int, c_ptr, c_ptr, c_ptr, c_ptr, c_size_t, c_ptr]),
+    "vt_mx_glm_value": (c_int, [c_int, c_int, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_ptr, c_ptr, c_dbl, c_i64,
+                                c_int, c_ptr, c_ptr, c_size_t, c_ptr]),
+    "vt_mx_glm_hvp": (c_int, [c_int, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_dbl, c_ptr, c_i64, c_int, c_ptr, c_ptr,
+                              c_size_t, c_ptr]),
+    "vt_mx_gemv": (c_int, [c_int, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_int, c_ptr, c_ptr, c_size_t, c_ptr]),
+    "vt_mx_gemv_t": (c_int, [c_int, c_ptr, c_i64, c_ptr, c_i64, c_ptr, c_ptr, c_i64, c_int, c_ptr, c_ptr, c_size_t,
+                             c_ptr]),
+    "vt_mx_gemm_nt_workspace_bytes": (c_size_t, [c_i64, c_i64, c_int]),
+    "vt_mx_gemm_nt": (c_int, [c_ptr, c_i64, c_ptr, c_i64, c_i64, c_ptr, c_i64, c_ptr, c_i64, c_i64, c_int,
+                              ctypes.c_float, c_ptr, c_int, c_ptr, c_i64, c_ptr, c_size_t, c_ptr]),
+    "vt_mx_gemm_tn_workspace_bytes": (c_size_t, [c_i64, c_int, c_int]),
+    "vt_mx_gemm_tn": (c_int, [c_int, c_ptr, c_i64, c_ptr, c_i64, c_int, c_int, c_ptr, c_i64, c_int, c_ptr, c_i64,
+                              ctypes.c_float, c_ptr, c_ptr, c_i64, c_ptr, c_size_t, c_ptr]),
     "vt_synth_normal": (c_int, [ctypes.c_uint64, ctypes.c_uint, c_i64, c_i64, c_int, c_ptr, c_i64, c_ptr]),
     "vt_synth_normal_f32": (c_int, [ctypes.c_uint64, ctypes.c_uint, c_i64, c_i64, c_int, c_ptr, c_i64, c_ptr]),
     "vt_synth_response": (c_int, [ctypes.c_uint64, c_i64, c_i64, c_int, c_ptr, c_ptr, c_ptr]),

@@ -1,0 +1,239 @@
+// Compact rows: quantisation and reading back.  Both stream: every input byte is read once, every output byte written
+// once, nothing else is moved.
+//
+// Scale of a block with largest magnitude a = m 2^f, 1 <= m < 2: a / 2^e has to round to a finite code.  E4M3 ends at
+// 448 = 1.75 2^8 and the next step would be 480: e = f - 8, one more if m 2^8 > 464 (the tie at 464 goes to 448, whose
+// last mantissa bit is 0).  E2M1 ends at 6 = 1.5 2^2 and the next step would be 8: e = f - 2, one more if
+// m 2^2 >= 7 (6's last bit is 1: the tie goes to 8).  Dividing by 2^e is exact, so a code carries ONE rounding: at most
+// half a step, 2^-4 (E4M3) or 2^-2 (E2M1) of the element's own size, or half the smallest step of its block.
+#include "vt_mx.h"
+#include <type_traits>
+
+namespace {
+
+typedef _Float16 f16;
+typedef __bf16 bf16;
+
+// Eight elements a thread, four threads a block of 32.
+constexpr int kPer = 8;
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int valid, bool vec, T (&x)[kPer]) {
+    if (vec && valid == kPer) {
+        constexpr int W = (int)sizeof(T) * kPer / 16;
+        u32x4 t[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) t[i] = ((const u32x4*)p)[i];
+        __builtin_memcpy(x, t, sizeof(t));
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) x[i] = i < valid ? p[i] : (T)0.0f;
+    }
+}
+
+// Exact bits of |x| in the order of the magnitudes; NaN above infinity.
+__device__ __forceinline__ uint64_t mag_bits(double x) { return __builtin_bit_cast(uint64_t, x) & ~(1ull << 63); }
+__device__ __forceinline__ unsigned mag_bits(float x) { return __builtin_bit_cast(unsigned, x) & 0x7fffffffu; }
+__device__ __forceinline__ uint64_t shfl_max(uint64_t v, int m) {
+    uint64_t o = __shfl_xor((unsigned long long)v, m, 64);
+    return o > v ? o : v;
+}
+__device__ __forceinline__ unsigned shfl_max(unsigned v, int m) {
+    unsigned o = __shfl_xor(v, m, 64);
+    return o > v ? o : v;
+}
+
+// Exponent e of the scale for the largest magnitude's bits, or 128: the block cannot be stored (NaN).
+template <int FMT>
+__device__ __forceinline__ int scale_exp(unsigned a) {
+    if (a >= 0x7f800000u) return 128;
+    const unsigned m = a & 0x7fffffu;
+    const int f = (int)(a >> 23) - 127;      // a subnormal's true exponent is lower still: the clamp takes both
+    const int e = FMT == VT_MX_FP8 ? f - 8 + (m > 0x680000u) : f - 2 + (m >= 0x600000u);
+    return e < -127 ? -127 : e;
+}
+template <int FMT>
+__device__ __forceinline__ int scale_exp(uint64_t a) {
+    if (a >= 0x47effffff0000000ull) return 128;      // 2^128 (1 - 2^-25) and up round to a float infinity
+    const uint64_t m = a & 0xfffffffffffffull;
+    const int f = (int)(a >> 52) - 1023;
+    const int e = FMT == VT_MX_FP8 ? f - 8 + (m > 0xd000000000000ull) : f - 2 + (m >= 0xc000000000000ull);
+    return e < -127 ? -127 : e;
+}
+
+// x 2^-e as a float whose rounding to a code is that of the exact number.
+__device__ __forceinline__ float scaled(float x, int e) { return x * __builtin_bit_cast(float, (unsigned)(127 - e) << 23); }
+__device__ __forceinline__ float scaled(double x, int e) {
+    // a double: rounded to odd, so that the second rounding (to 4 bits or fewer) sees which side of a tie it is on
+    const double y = x * __builtin_bit_cast(double, (uint64_t)(1023 - e) << 52);
+    float f = (float)y;
+    if ((double)f != y) {
+        unsigned b = __builtin_bit_cast(unsigned, f);
+        if (fabs((double)f) > fabs(y)) --b;
+        f = __builtin_bit_cast(float, b | 1u);
+    }
+    return f;
+}
+template <typename T>
+__device__ __forceinline__ float scaled(T x, int e) { return scaled((float)x, e); }
+
+template <int FMT>
+__device__ __forceinline__ void store_codes(uint8_t* p, const float (&v)[kPer]) {
+    if constexpr (FMT == VT_MX_FP8) {
+        u32x2 w;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            int t = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i], v[4 * i + 1], 0, false);
+            w[i] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2], v[4 * i + 3], t, true);
+        }
+        *(u32x2*)p = w;
+    } else {
+        unsigned w = 0;
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0], v[1], 1.0f, 0);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2], v[3], 1.0f, 1);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4], v[5], 1.0f, 2);
+        w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6], v[7], 1.0f, 3);
+        *(unsigned*)p = w;
+    }
+}
+
+// blockDim = (tx, 256 / tx): tx threads along a row's groups of eight, the rest along rows.
+template <int FMT, typename T>
+__global__ __launch_bounds__(256) void k_mx_quantise(const T* X, int64_t ldx, int64_t N, int D, bool vec, uint8_t* codes,
+                                                     int64_t ldc, uint8_t* scales, int64_t lds) {
+    const int groups = mx_blocks(D) * 4;
+    const int g = blockIdx.x * blockDim.x + threadIdx.x;
+    if (g >= groups) return;                  // groups is a multiple of 4: the four threads of a block leave together
+    const int c0 = g * kPer;
+    const int valid = D - c0 < 0 ? 0 : (D - c0 < kPer ? D - c0 : kPer);
+    for (int64_t n = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; n < N; n += (int64_t)gridDim.y * blockDim.y) {
+        T x[kPer];
+        load8(X + n * ldx + c0, valid, vec, x);
+        using M = typename std::conditional<sizeof(T) == 8, double, float>::type;
+        auto a = mag_bits((M)x[0]);
+#pragma unroll
+        for (int i = 1; i < kPer; ++i) {
+            const auto b = mag_bits((M)x[i]);
+            a = b > a ? b : a;
+        }
+        a = shfl_max(a, 1);
+        a = shfl_max(a, 2);
+        const int e = scale_exp<FMT>(a);
+        float v[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) v[i] = e == 128 ? 0.0f : scaled(x[i], e);
+        store_codes<FMT>(codes + n * ldc + (int64_t)g * (FMT == VT_MX_FP8 ? 8 : 4), v);
+        if ((g & 3) == 0) scales[n * lds + (g >> 2)] = (uint8_t)(e + 127);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int valid, bool vec, const float (&v)[kPer]) {
+    T x[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) x[i] = (T)v[i];
+    if (vec && valid == kPer) {
+        constexpr int W = (int)sizeof(T) * kPer / 16;
+        u32x4 t[W];
+        __builtin_memcpy(t, x, sizeof(t));
+#pragma unroll
+        for (int i = 0; i < W; ++i) ((u32x4*)p)[i] = t[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            if (i < valid) p[i] = x[i];
+    }
+}
+
+template <int FMT, typename T>
+__global__ __launch_bounds__(256) void k_mx_dequantise(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds,
+                                                       int64_t N, int D, bool vec, T* out, int64_t ldo) {
+    const int g = blockIdx.x * blockDim.x + threadIdx.x;
+    const int c0 = g * kPer;
+    if (c0 >= D) return;
+    const int valid = D - c0 < kPer ? D - c0 : kPer;
+    for (int64_t n = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; n < N; n += (int64_t)gridDim.y * blockDim.y) {
+        const float s = mx_scale(scales[n * lds + (g >> 2)]);
+        float v[kPer];
+        if constexpr (FMT == VT_MX_FP8) {
+            const u32x2 w = *(const u32x2*)(codes + n * ldc + (int64_t)g * 8);
+            float t[4];
+            mx_word<FMT>(w[0], s, t);
+            v[0] = t[0], v[1] = t[1], v[2] = t[2], v[3] = t[3];
+            mx_word<FMT>(w[1], s, t);
+            v[4] = t[0], v[5] = t[1], v[6] = t[2], v[7] = t[3];
+        } else {
+            mx_word<FMT>(*(const unsigned*)(codes + n * ldc + (int64_t)g * 4), s, v);
+        }
+        store8(out + n * ldo + c0, valid, vec, v);
+    }
+}
+
+// Threads along the row: the power of two that covers its groups of eight, 256 at most.
+void stream_shape(int groups, int64_t N, dim3& grid, dim3& block) {
+    int tx = 4;
+    while (tx < groups && tx < 256) tx *= 2;
+    const int ty = 256 / tx;
+    const int64_t rows = (N + ty - 1) / ty;
+    block = dim3(tx, ty);
+    grid = dim3((groups + tx - 1) / tx, (unsigned)std::min<int64_t>(rows, 65535));
+}
+
+template <int FMT, typename T>
+int quantise(const void* X, int64_t ldx, int64_t N, int D, void* codes, int64_t ldc, void* scales, int64_t lds, hipStream_t st) {
+    dim3 grid, block;
+    stream_shape(mx_blocks(D) * 4, N, grid, block);
+    const bool vec = (uintptr_t)X % 16 == 0 && ldx * (int64_t)sizeof(T) % 16 == 0;
+    hipLaunchKernelGGL((k_mx_quantise<FMT, T>), grid, block, 0, st, (const T*)X, ldx, N, D, vec, (uint8_t*)codes, ldc,
+                       (uint8_t*)scales, lds);
+    return vt_launch_status();
+}
+
+template <int FMT, typename T>
+int dequantise(const void* codes, int64_t ldc, const void* scales, int64_t lds, int64_t N, int D, void* out, int64_t ldo,
+               hipStream_t st) {
+    dim3 grid, block;
+    stream_shape(mx_blocks(D) * 4, N, grid, block);
+    const bool vec = (uintptr_t)out % 16 == 0 && ldo * (int64_t)sizeof(T) % 16 == 0;
+    hipLaunchKernelGGL((k_mx_dequantise<FMT, T>), grid, block, 0, st, (const uint8_t*)codes, ldc, (const uint8_t*)scales, lds,
+                       N, D, vec, (T*)out, ldo);
+    return vt_launch_status();
+}
+
+}  // namespace
+
+extern "C" int vt_mx_quantise(int type, const void* X, int64_t ldx, int64_t N, int D, int format, void* codes, int64_t ldc,
+                              void* scales, int64_t lds, void* stream) {
+    if (!mx_rows_ok(format, codes, ldc, scales, lds, N, D) || type < VT_TYPE_F64 || type > VT_TYPE_F16) return VT_ERR_BAD_ARG;
+    if (N == 0) return VT_OK;
+    if (!X || ldx < D) return VT_ERR_BAD_ARG;
+    hipStream_t st = (hipStream_t)stream;
+#define VT_QUANT(T) \
+    (format == VT_MX_FP8 ? quantise<VT_MX_FP8, T>(X, ldx, N, D, codes, ldc, scales, lds, st) \
+                         : quantise<VT_MX_FP4, T>(X, ldx, N, D, codes, ldc, scales, lds, st))
+    switch (type) {
+        case VT_TYPE_F64: return VT_QUANT(double);
+        case VT_TYPE_F32: return VT_QUANT(float);
+        case VT_TYPE_BF16: return VT_QUANT(bf16);
+        default: return VT_QUANT(f16);
+    }
+#undef VT_QUANT
+}
+
+extern "C" int vt_mx_dequantise(int format, const void* codes, int64_t ldc, const void* scales, int64_t lds, int64_t N, int D,
+                                int type, void* out, int64_t ldo, void* stream) {
+    if (!mx_rows_ok(format, codes, ldc, scales, lds, N, D) || type < VT_TYPE_F64 || type > VT_TYPE_F16) return VT_ERR_BAD_ARG;
+    if (N == 0) return VT_OK;
+    if (!out || ldo < D) return VT_ERR_BAD_ARG;
+    hipStream_t st = (hipStream_t)stream;
+#define VT_DEQUANT(T) \
+    (format == VT_MX_FP8 ? dequantise<VT_MX_FP8, T>(codes, ldc, scales, lds, N, D, out, ldo, st) \
+                         : dequantise<VT_MX_FP4, T>(codes, ldc, scales, lds, N, D, out, ldo, st))
+    switch (type) {
+        case VT_TYPE_F64: return VT_DEQUANT(double);
+        case VT_TYPE_F32: return VT_DEQUANT(float);
+        case VT_TYPE_BF16: return VT_DEQUANT(bf16);
+        default: return VT_DEQUANT(f16);
+    }
+#undef VT_DEQUANT
+}

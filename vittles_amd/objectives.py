@@ -10,7 +10,7 @@ methods of the objective, computed in closed form on the device.
 import numpy as np
 import torch
 
-from . import _lib, device as dev, sharding
+from . import _lib, compact, device as dev, sharding
 
 
 class RegisteredObjective:
@@ -93,23 +93,40 @@ class WeightedGLMObjective(RegisteredObjective):
     up to 128 the f32-MFMA resident kernels, beyond the tiled kernels on float panels with fp64 products and a
     slab-wise fp64 solve (configs[2]'s D = 1000 with X and S at half the footprint).  Row operators (link, gradient,
     value, HVP and the CG route, A v, A^T u): D <= 20448, rows are re-laid on a 16-byte pitch here (configs[3]'s
-    D = 20000 on a float X)."""
+    D = 20000 on a float X).
+
+    ``dtype="mxfp8"`` / ``"mxfp4"``, or ``X`` given as ``compact.CompactRows``: COMPACT storage, 8 or 4 bits a feature
+    with a scale for every 32 of them.  All row operators (link, gradient, value, HVP and the CG route, A v, A^T u) read
+    the compact rows, at any D, with every vector and sum in double; they compute the objective OF THE STORED values
+    exactly.  There is no Hessian route: ``solver_lib.get_cg_solver`` on ``cg.GLMHessianVectorProduct`` solves."""
 
     def __init__(self, X, y, family="logistic", prior=None, scale=1.0, offset=None,
                  device=None, process_group=None, dtype=torch.float64):
         dev.require_gpu()
         if family not in _lib.FAMILY:
             raise ValueError("family must be one of %s" % (tuple(_lib.FAMILY),))
-        if dtype not in (torch.float64, torch.float32):
-            raise ValueError("dtype must be torch.float64 or torch.float32")
+        if isinstance(X, compact.CompactRows):
+            if dtype not in (torch.float64, X.format):          # torch.float64: the default, not asked for
+                raise ValueError("X is stored in %s already: dtype cannot be %s" % (X.format, dtype))
+            if device is not None and torch.device(device) != X.device:
+                raise ValueError("X is on %s already" % X.device)
+            dtype = X.format
+        if dtype not in (torch.float64, torch.float32) + compact.FORMATS:
+            raise ValueError("dtype must be torch.float64 or torch.float32 (or a compact format: %s)"
+                             % ", ".join(compact.FORMATS))
         self.family = family
         self.dtype = dtype
-        self.X = dev.to_device(X, device, dtype=dtype)
-        if self.X.ndim != 2:
-            raise ValueError("X must be (N, D)")
-        if self.X.shape[0] > 0 and self.X.stride(1) != 1:
-            self.X = self.X.contiguous()
-        self.X = _aligned_rows(self.X)
+        if isinstance(X, compact.CompactRows):
+            self.X = X
+        elif dtype in compact.FORMATS:
+            self.X = compact.quantise(X, dtype, device=device)
+        else:
+            self.X = dev.to_device(X, device, dtype=dtype)
+            if self.X.ndim != 2:
+                raise ValueError("X must be (N, D)")
+            if self.X.shape[0] > 0 and self.X.stride(1) != 1:
+                self.X = self.X.contiguous()
+            self.X = _aligned_rows(self.X)
         self.N, self.D = self.X.shape
         self.device = self.X.device
         self.y = dev.to_device(y, self.device).contiguous()
@@ -147,6 +164,9 @@ class WeightedGLMObjective(RegisteredObjective):
         """One pass over X: returns dict(H, g, r, d) of CUDA tensors (cached for the
         last (theta, w) pair so grad()/hessian()/cross_hessian() share one pass)."""
         lib = dev.require_gpu()
+        if isinstance(self.X, compact.CompactRows):
+            raise _lib.VittlesHipError("compact rows (%s) have no Hessian route: solve with solver_lib.get_cg_solver on "
+                                       "cg.GLMHessianVectorProduct" % self.dtype)
         theta = dev.to_device(theta, self.device).contiguous()
         w = dev.to_device(w, self.device).contiguous()
         if theta.shape != (self.D,):
@@ -194,9 +214,10 @@ class WeightedGLMObjective(RegisteredObjective):
         return out
 
     def grad(self, opt, hyper):
-        if self.dtype == torch.float32:
-            # fp32 mode: the fused kernel's gradient is summed in f32 per wave (~1e-6 of sum |terms|), too coarse
-            # for an optimiser's stopping test; the row kernel carries the sum in fp64 (one more pass over X)
+        if self.dtype != torch.float64:
+            # compact rows have no fused kernel; fp32 mode: the fused kernel's gradient is summed in f32 per wave
+            # (~1e-6 of sum |terms|), too coarse for an optimiser's stopping test; the row kernel carries the sum in
+            # fp64 (one more pass over X)
             from . import rows
             g, _, _ = rows.glm_grad(self, opt, hyper, prior=self.prior if self._rank() == 0 else None)
             return self._all_reduce(g)

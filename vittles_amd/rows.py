@@ -1,7 +1,8 @@
-"""Host wrappers over the row-streaming kernels (vt_rows.hip): K0, K3, K6, K9, value."""
+"""Host wrappers over the row-streaming kernels (vt_rows.hip; vt_mx_rows.hip for compact rows): K0, K3, K6, K9, value."""
 import torch
 
 from . import _lib, device as dev
+from .compact import CompactRows, TYPE as _MX_TYPE, on_device
 
 _ws_cache = {}
 
@@ -48,7 +49,41 @@ def _rowmajor(A):
     return A if (A.stride(1) == 1 or A.shape[0] == 0) else A.contiguous()
 
 
+def _vector(t, n, X, what):
+    """A vector that goes with compact rows ``X``, checked: the kernels take its address."""
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float64 or t.shape != (n,) or t.device != X.device:
+        raise ValueError("%s must be a float64 tensor of shape (%d,) on %s" % (what, n, X.device))
+    return t.contiguous()
+
+
+def _compact(name, X, lead, tail):
+    """``vt_mx_<name>`` on compact rows: (lead, format, codes, ldc, scales, lds, tail, workspace, stream).  The workspace
+    belongs to the call (and, under capture, to the graph): two graphs never share one."""
+    lib = dev.require_gpu()
+    with on_device(X.device):
+        nbytes = lib.vt_mx_rows_workspace_bytes(*X.shape)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=X.device)
+        _lib.check(getattr(lib, "vt_mx_" + name)(*lead, X.c_format(), *X.c_args(), *tail, ws.data_ptr(), nbytes,
+                                                 dev.stream_ptr()), "vt_mx_" + name)
+
+
+def _compact_glm(name, obj, theta, w, outs, prior=()):
+    """A GLM operator on the compact rows of ``obj``; ``outs``: the tensors (or None) that it fills."""
+    X = obj.X
+    theta = _vector(dev.to_device(theta, obj.device), obj.D, X, "opt_par")
+    w = _vector(dev.to_device(w, obj.device), obj.N, X, "hyper_par (data weights)")
+    if obj.offset is not None:
+        _vector(obj.offset, obj.N, X, "offset")
+    _compact(name, X, (_lib.FAMILY[obj.family],),
+             (theta.data_ptr(), obj.y.data_ptr(), w.data_ptr(), dev.ptr(obj.offset), obj.scale,
+              *(dev.ptr(p) for p in prior), obj.N, obj.D, *(dev.ptr(t) for t in outs)))
+
+
 def _fp64_only(A, what):
+    if isinstance(A, CompactRows):
+        raise _lib.VittlesHipError(
+            "%s is not part of the compact storage modes (they cover link, gradient, HVP, value, A v, A^T u, the CG route and "
+            "the products of rows.gemm_nt / rows.gemm_tn): build the objective with dtype=torch.float64" % what)
     if A.dtype != torch.float64:
         raise _lib.VittlesHipError(
             "%s is not part of the fp32 storage mode (it covers the Hessian, the sensitivity solve, predictions, gradient, HVP, "
@@ -56,7 +91,9 @@ def _fp64_only(A, what):
 
 
 def gemv_t(A, u):
-    """out (D,) = A^T u for a row-major (N, D) CUDA tensor A (K9)."""
+    """out (D,) = A^T u for a row-major (N, D) CUDA tensor A or ``CompactRows`` (K9)."""
+    if isinstance(A, CompactRows):
+        return gemv_t2(A, u, None)
     lib = dev.require_gpu()
     A = _rowmajor(A)
     N, D = A.shape
@@ -69,7 +106,12 @@ def gemv_t(A, u):
 
 
 def gemv(A, v):
-    """out (N,) = A v for a row-major (N, D) CUDA tensor A."""
+    """out (N,) = A v for a row-major (N, D) CUDA tensor A or ``CompactRows``."""
+    if isinstance(A, CompactRows):
+        v = _vector(v, A.D, A, "v")
+        out = torch.empty(A.shape[0], dtype=torch.float64, device=A.device)
+        _compact("gemv", A, (), (v.data_ptr(), *A.shape, out.data_ptr()))
+        return out
     lib = dev.require_gpu()
     A = _rowmajor(A)
     N, D = A.shape
@@ -82,7 +124,13 @@ def gemv(A, v):
 
 
 def gemv_t2(A, u1, u2):
-    """out (D,) = A^T (u1 .* u2) for a row-major (N, D) CUDA tensor A."""
+    """out (D,) = A^T (u1 .* u2) for a row-major (N, D) CUDA tensor A or ``CompactRows``."""
+    if isinstance(A, CompactRows):
+        u1 = _vector(u1, A.shape[0], A, "u1")
+        u2 = None if u2 is None else _vector(u2, A.shape[0], A, "u2")
+        out = torch.empty(A.D, dtype=torch.float64, device=A.device)
+        _compact("gemv_t", A, (), (u1.data_ptr(), dev.ptr(u2), *A.shape, out.data_ptr()))
+        return out
     lib = dev.require_gpu()
     A = _rowmajor(A)
     N, D = A.shape
@@ -158,7 +206,13 @@ _tn_ws_cache = {}
 
 def gemm_tn(A, B, rowscale=None, alpha=1.0, bias=None, out=None):
     """out (Da, Db) = alpha * A^T diag(rowscale) B + bias[None, :] for row-major CUDA tensors
-    A (N, Da), B (N, Db): K9 for many weight vectors at once (fp64 MFMA, split over N)."""
+    A (N, Da), B (N, Db): K9 for many weight vectors at once (fp64 MFMA, split over N).
+
+    ``A`` as ``CompactRows``: the gradient of a linear layer's weights from its stored activations.  ``B`` (the gradient
+    of the layer's outputs) is float32, bfloat16 or float16, ``rowscale`` float64, ``bias`` float32; products are exact,
+    sums and ``out`` float32."""
+    if isinstance(A, CompactRows):
+        return _compact_gemm_tn(A, B, rowscale, alpha, bias, out)
     lib = dev.require_gpu()
     _fp64_only(A, "gemm_tn (first operand)")
     if B.dtype not in (torch.float64, torch.float32):
@@ -187,6 +241,66 @@ def gemm_tn(A, B, rowscale=None, alpha=1.0, bias=None, out=None):
     return out
 
 
+def _matrix_out(out, shape, dtypes, device):
+    """``out`` of a float product, checked, or a new tensor of the first type."""
+    if out is None:
+        return torch.empty(shape, dtype=dtypes[0], device=device)
+    if out.shape != shape or out.dtype not in dtypes or out.device != device or (out.numel() and (
+            out.stride(1) != 1 and out.shape[1] > 1 or dev.ld(out) < shape[1])):
+        raise ValueError("out must be a %s row-major tensor of %s on %s" % (shape, " or ".join(map(str, dtypes)), device))
+    return out
+
+
+def _bias(bias, n, device):
+    if bias is None:
+        return None
+    if bias.dtype != torch.float32 or bias.shape != (n,) or bias.device != device:
+        raise ValueError("bias must be a float32 tensor of shape (%d,) on %s" % (n, device))
+    return bias.contiguous()
+
+
+def _compact_gemm_tn(A, B, rowscale, alpha, bias, out):
+    lib = dev.require_gpu()
+    N, Da = A.shape
+    if B.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError("gemm_tn: B must be float32, bfloat16 or float16 beside compact rows")
+    if B.ndim != 2 or B.shape[0] != N or B.shape[1] < 1 or B.device != A.device:
+        raise ValueError("A and B must have the same number of rows and device, B at least one column")
+    Db = B.shape[1]
+    if N > 0 and (B.stride(1) != 1 or dev.ld(B) < Db):
+        B = B.contiguous()
+    rowscale = None if rowscale is None else _vector(rowscale, N, A, "rowscale")
+    bias = _bias(bias, Db, A.device)
+    out = _matrix_out(out, (Da, Db), (torch.float32,), A.device)
+    with on_device(A.device):
+        nbytes = lib.vt_mx_gemm_tn_workspace_bytes(N, Da, Db)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=A.device)
+        _lib.check(lib.vt_mx_gemm_tn(A.c_format(), *A.c_args(), Da, _MX_TYPE[B.dtype], B.data_ptr(), dev.ld(B), Db,
+                                     dev.ptr(rowscale), N, float(alpha), dev.ptr(bias), out.data_ptr(), dev.ld(out),
+                                     ws.data_ptr(), nbytes, dev.stream_ptr()), "vt_mx_gemm_tn")
+    return out
+
+
+def gemm_nt(A, B, alpha=1.0, bias=None, out=None):
+    """out (M, N) = alpha * A B^T + bias[None, :] for 4-bit ``CompactRows`` A (M, K), B (N, K): the scores of all pairs of
+    rows, on the scaled MFMA.  Sums in float32; ``out`` float32 (new if not given) or bfloat16, ``bias`` (N,) float32."""
+    if not (isinstance(A, CompactRows) and isinstance(B, CompactRows) and A.format == B.format == "mxfp4"):
+        raise TypeError("gemm_nt: A and B must be CompactRows in mxfp4")
+    if A.D != B.D or A.device != B.device:
+        raise ValueError("A and B must have the same number of columns and device")
+    lib = dev.require_gpu()
+    M, N = A.shape[0], B.shape[0]
+    bias = _bias(bias, N, A.device)
+    out = _matrix_out(out, (M, N), (torch.float32, torch.bfloat16), A.device)
+    with on_device(A.device):
+        nbytes = lib.vt_mx_gemm_nt_workspace_bytes(M, N, A.D)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=A.device)
+        _lib.check(lib.vt_mx_gemm_nt(*A.c_args(), M, *B.c_args(), N, A.D, float(alpha), dev.ptr(bias),
+                                     _MX_TYPE[out.dtype], out.data_ptr(), dev.ld(out), ws.data_ptr(), nbytes,
+                                     dev.stream_ptr()), "vt_mx_gemm_nt")
+    return out
+
+
 def gemm_tn_tiled(A, B, tile=8192):
     """``A^T B`` for operands of ANY width: vt_gemm_tn takes at most 8192 columns per operand, so wider ones are cut
     into column panels and every (panel of A, panel of B) pair is one vt_gemm_tn call into its slice of the result
@@ -211,6 +325,9 @@ def glm_link(obj, theta, w, want_z=False):
     z = torch.empty(obj.N, dtype=torch.float64, device=obj.device) if want_z else None
     r = torch.empty(obj.N, dtype=torch.float64, device=obj.device)
     d = torch.empty(obj.N, dtype=torch.float64, device=obj.device)
+    if isinstance(obj.X, CompactRows):
+        _compact_glm("glm_link", obj, theta, w, (z, r, d))
+        return z, r, d
     ws = _workspace(obj.D, obj.device)
     _lib.check(_lib.fn(lib, "vt_glm_link", obj.X)(_lib.FAMILY[obj.family], obj.X.data_ptr(), dev.ld(obj.X), theta.data_ptr(),
                                obj.y.data_ptr(), w.data_ptr(), dev.ptr(obj.offset), obj.scale, obj.N, obj.D,
@@ -227,6 +344,10 @@ def glm_grad(obj, theta, w, prior=None):
     g = torch.empty(obj.D, dtype=torch.float64, device=obj.device)
     r = torch.empty(obj.N, dtype=torch.float64, device=obj.device)
     d = torch.empty(obj.N, dtype=torch.float64, device=obj.device)
+    if isinstance(obj.X, CompactRows):
+        prior = None if prior is None else _vector(prior, obj.D, obj.X, "prior")
+        _compact_glm("glm_grad", obj, theta, w, (g, r, d), prior=(prior,))
+        return g, r, d
     ws = _workspace(obj.D, obj.device)
     _lib.check(_lib.fn(lib, "vt_glm_grad", obj.X)(_lib.FAMILY[obj.family], obj.X.data_ptr(), dev.ld(obj.X), theta.data_ptr(),
                                obj.y.data_ptr(), w.data_ptr(), dev.ptr(obj.offset), obj.scale, dev.ptr(prior),
@@ -236,9 +357,18 @@ def glm_grad(obj, theta, w, prior=None):
 
 
 def glm_hvp(X, d, v, prior=None, prior_scalar=0.0, out=None):
-    """K6: out = X^T (d .* (X v)) + prior .* v."""
-    lib = dev.require_gpu()
+    """K6: out = X^T (d .* (X v)) + prior .* v for a row-major (N, D) CUDA tensor X or ``CompactRows``."""
     N, D = X.shape
+    if isinstance(X, CompactRows):
+        d, v = _vector(d, N, X, "d"), _vector(v, D, X, "v")
+        prior = None if prior is None else _vector(prior, D, X, "prior")
+        if out is None:
+            out = torch.empty(D, dtype=torch.float64, device=X.device)
+        elif out.dtype != torch.float64 or out.shape != (D,) or out.device != X.device or not out.is_contiguous():
+            raise ValueError("out must be a contiguous float64 tensor of shape (%d,) on %s" % (D, X.device))
+        _compact("glm_hvp", X, (), (d.data_ptr(), dev.ptr(prior), float(prior_scalar), v.data_ptr(), N, D, out.data_ptr()))
+        return out
+    lib = dev.require_gpu()
     if out is None:
         out = torch.empty(D, dtype=torch.float64, device=X.device)
     ws = _workspace(D, X.device)
@@ -280,10 +410,13 @@ def glm_value(obj, theta, w):
     theta = dev.to_device(theta, obj.device).contiguous()
     w = dev.to_device(w, obj.device).contiguous()
     val = torch.empty(1, dtype=torch.float64, device=obj.device)
-    ws = _workspace(obj.D, obj.device)
-    _lib.check(_lib.fn(lib, "vt_glm_value", obj.X)(_lib.FAMILY[obj.family], obj.X.data_ptr(), dev.ld(obj.X), theta.data_ptr(),
-                                obj.y.data_ptr(), w.data_ptr(), dev.ptr(obj.offset), obj.scale, obj.N, obj.D,
-                                val.data_ptr(), ws.data_ptr(), ws.numel() * 8, dev.stream_ptr()), "vt_glm_value")
+    if isinstance(obj.X, CompactRows):
+        _compact_glm("glm_value", obj, theta, w, (val,))
+    else:
+        ws = _workspace(obj.D, obj.device)
+        _lib.check(_lib.fn(lib, "vt_glm_value", obj.X)(_lib.FAMILY[obj.family], obj.X.data_ptr(), dev.ld(obj.X), theta.data_ptr(),
+                                    obj.y.data_ptr(), w.data_ptr(), dev.ptr(obj.offset), obj.scale, obj.N, obj.D,
+                                    val.data_ptr(), ws.data_ptr(), ws.numel() * 8, dev.stream_ptr()), "vt_glm_value")
     obj._all_reduce(val)
     total = float(val.item())
     if obj.prior is not None:
