@@ -1,8 +1,15 @@
 // Row operators on compact rows: link, gradient, value, fused HVP, A v and A^T (u1 .* u2), with fp64 vectors and sums.
 //     for every row n:  dot_n = x_n . v,  t_n = op(dot_n, per-row scalars) -> per-row outputs,  out += t_n x_n
-// Two passes: one wave per row takes the dots and leaves t_n in the workspace; then every thread owns eight columns and
-// walks a slab of rows.  Partial sums are combined in a fixed order (no atomics: the same bits every time).
+// One pass: a team of threads holds the codes of R rows in registers from the dot to the column sums, 16 columns
+// ("a piece": half a block, 16 bytes of E4M3 or 8 of E2M1) a thread and round, and their sums of the columns for the
+// whole kernel.  Partial sums are combined in a fixed order (no atomics: the same bits every time).
+// Bound: HBM for E4M3 (reads alone: 5.4 - 5.9 TB/s), the VALU for E2M1.  An element costs half a conversion to float and
+// one to double, once if its double is kept and twice if not, and two fp64 FMAs: 3.5 to 5 instructions of 4 cycles for 64
+// elements, and about 100 more a round for the sums.  Measured, HVP in TB/s of stored bytes: E4M3 N = 4 10^6, D = 100 5.1;
+// N = 10^5, D = 8192 4.8, D = 20 000 4.1 (503 us); E2M1 3.2, 2.6, 2.6 (405 us).
 #include "vt_mx.h"
+#include <type_traits>
+#include <utility>
 
 namespace {
 
@@ -24,30 +31,416 @@ struct MxRows {
     double* part;                  // [slabs][D]
 };
 
-// The row's coefficient in the column sum; writes the row's outputs.
+// The row's scalars, fetched a round before they are used.
+struct RowScal {
+    double y, w, off;
+};
 template <int OP>
-__device__ __forceinline__ double mx_row_op(const MxRows& a, int64_t n, double dot) {
+__device__ __forceinline__ RowScal row_scal(const MxRows& a, int64_t n) {
+    RowScal s{0.0, 0.0, 0.0};
+    if constexpr (OP == OP_GEMV) return s;
+    s.y = a.y[n];
+    if constexpr (OP == OP_GEMVT) s.w = a.w ? a.w[n] : 1.0;
+    if constexpr (OP == OP_LINK || OP == OP_GRAD || OP == OP_VALUE) {
+        s.w = a.w[n];
+        if (a.offset) s.off = a.offset[n];
+    }
+    return s;
+}
+
+// The row's coefficient in the column sum (VALUE: its loss); the leading lane writes the row's outputs.
+template <int OP>
+__device__ __forceinline__ double mx_row_op(const MxRows& a, int64_t n, const RowScal& s, double dot, bool lead) {
     if constexpr (OP == OP_GEMVT) {
-        return a.w ? a.y[n] * a.w[n] : a.y[n];
+        return s.y * s.w;
     } else if constexpr (OP == OP_HVP) {
-        return a.y[n] * dot;
+        return s.y * dot;
     } else if constexpr (OP == OP_GEMV) {
-        a.z[n] = dot;
+        if (lead) a.z[n] = dot;
         return 0.0;
     } else {
-        const double z = dot + (a.offset ? a.offset[n] : 0.0), w = a.w[n];
+        const double z = dot + s.off;
         if constexpr (OP == OP_VALUE) {
-            return w * vt_loss(a.family, z, a.y[n]);
+            return s.w * vt_loss(a.family, z, s.y);
         } else {
             double l1, l2;
-            vt_link(a.family, z, a.y[n], l1, l2);
-            if (a.z) a.z[n] = z;
-            if (a.r) a.r[n] = a.scale * l1;
-            if (a.d) a.d[n] = a.scale * w * l2;
-            return w * (a.scale * l1);
+            vt_link(a.family, z, s.y, l1, l2);
+            if (lead) {
+                if (a.z) a.z[n] = z;
+                if (a.r) a.r[n] = a.scale * l1;
+                if (a.d) a.d[n] = a.scale * s.w * l2;
+            }
+            return s.w * (a.scale * l1);
         }
     }
 }
+
+// ---- one pass ---------------------------------------------------------------------------------------------------------
+// Codes and scales come through buffer descriptors that begin at a workgroup's rows of the round and end with the
+// matrix: the lane's offset is 32 bits, and rows behind the end read as 0 (their coefficient is 0 too).
+typedef __amdgpu_buffer_rsrc_t MxRsrc;
+__device__ __forceinline__ MxRsrc rows_rsrc(const uint8_t* base, int64_t n0, int64_t ld, int64_t N, int64_t width) {
+    const int64_t bytes = n0 < N ? (N - 1 - n0) * ld + width : 0;
+    const uint64_t p = (uint64_t)(base + n0 * ld);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)p), hi = __builtin_amdgcn_readfirstlane((uint32_t)(p >> 32));
+    return __builtin_amdgcn_make_buffer_rsrc((void*)(((uint64_t)hi << 32) | lo), 0,
+                                             __builtin_amdgcn_readfirstlane((uint32_t)std::min<int64_t>(bytes, 0xfffffff0)), 0x00020000);
+}
+
+template <int FMT> struct Piece;
+template <> struct Piece<VT_MX_FP8> {
+    typedef u32x4 type;
+    static __device__ __forceinline__ type load(MxRsrc r, unsigned off) {
+        return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0));
+    }
+};
+template <> struct Piece<VT_MX_FP4> {
+    typedef u32x2 type;
+    static __device__ __forceinline__ type load(MxRsrc r, unsigned off) {
+        return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
+    }
+};
+
+// Columns 2 p, 2 p + 1 of a piece.
+template <int FMT, int P>
+__device__ __forceinline__ f32x2 piece_pair(const typename Piece<FMT>::type& w, float scale) {
+    if constexpr (FMT == VT_MX_FP8) return mx_pair<FMT, P & 1>(w[P >> 1], scale);
+    else return mx_pair<FMT, P & 3>(w[P >> 2], scale);
+}
+
+typedef double f64x2 __attribute__((ext_vector_type(2)));
+
+template <int... I, typename F>
+__device__ __forceinline__ void each_impl(std::integer_sequence<int, I...>, F&& f) { (f(std::integral_constant<int, I>()), ...); }
+template <int N, typename F>
+__device__ __forceinline__ void each(F&& f) { each_impl(std::make_integer_sequence<int, N>(), f); }
+
+// The value of the lane's partner, for sums over pairs: lane ^ M for M = 1, 2, 8; lane ^ 7 for M = 4 (as good: it too
+// joins the lower and the upper half of eight).  DPP moves on the VALU, a tenth of the latency of a permutation through LDS.
+template <int M>
+__device__ __forceinline__ double partner(double v) {
+    constexpr int ctrl = M == 1 ? 0xb1 : M == 2 ? 0x4e : M == 4 ? 0x141 : 0x128;     // quad_perm, row_half_mirror, row_ror:8
+    const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), ctrl, 0xf, 0xf, true);
+    const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), ctrl, 0xf, 0xf, true);
+    return __hiloint2double(hi, lo);
+}
+// Lanes without bit M: the sum of a over the lane and lane ^ M; lanes with it: that of b (M = 16, 32).
+template <int M>
+__device__ __forceinline__ double swap_sum(double a, double b) {
+    unsigned al = __double2loint(a), ah = __double2hiint(a), bl = __double2loint(b), bh = __double2hiint(b);
+    if constexpr (M == 32) {
+        const auto l = __builtin_amdgcn_permlane32_swap(al, bl, false, false), h = __builtin_amdgcn_permlane32_swap(ah, bh, false, false);
+        return __hiloint2double(h[0], l[0]) + __hiloint2double(h[1], l[1]);
+    } else {
+        const auto l = __builtin_amdgcn_permlane16_swap(al, bl, false, false), h = __builtin_amdgcn_permlane16_swap(ah, bh, false, false);
+        return __hiloint2double(h[0], l[0]) + __hiloint2double(h[1], l[1]);
+    }
+}
+
+// d[r], r < R, summed over the T lanes of a team: the result is the sum of row lane / (T / R) of the team.  Halving: in
+// every step a lane gives away the half of its rows that its partner keeps.
+template <int T, int R>
+__device__ __forceinline__ double team_sum(const double (&d)[R], int lane) {
+    if constexpr (T == 1) {
+        return d[0];
+    } else if constexpr (T >= 32) {
+        if constexpr (R == 1) {
+            const double sum[1] = {swap_sum<T / 2>(d[0], d[0])};
+            return team_sum<T / 2, 1>(sum, lane);
+        } else {
+            double half[R / 2];
+#pragma unroll
+            for (int i = 0; i < R / 2; ++i) half[i] = swap_sum<T / 2>(d[i], d[i + R / 2]);
+            return team_sum<T / 2, R / 2>(half, lane);
+        }
+    } else if constexpr (R == 1) {
+        const double sum[1] = {d[0] + partner<T / 2>(d[0])};
+        return team_sum<T / 2, 1>(sum, lane);
+    } else {
+        double half[R / 2];
+        const bool up = lane & (T / 2);
+#pragma unroll
+        for (int i = 0; i < R / 2; ++i) {
+            const double keep = up ? d[i + R / 2] : d[i], give = up ? d[i] : d[i + R / 2];
+            half[i] = keep + partner<T / 2>(give);
+        }
+        return team_sum<T / 2, R / 2>(half, lane);
+    }
+}
+
+// Keeps the compiler from holding on to numbers that are cheaper to decode again.
+template <typename W>
+__device__ __forceinline__ void decode_again(W& w, float& s) {
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(W) / 4); ++i) {
+        unsigned u = w[i];
+        asm volatile("" : "+v"(u));
+        w[i] = u;
+    }
+    asm volatile("" : "+v"(s));
+}
+
+__device__ __forceinline__ double read_lane(double v, int lane) {
+    return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane), __builtin_amdgcn_readlane(__double2loint(v), lane));
+}
+
+// Rows of at most 16 T columns: T lanes of a wave a row, R rows a round; the round's numbers (decoded once, as doubles)
+// and the column sums in registers, v in LDS.  After the sums every lane has one row (T = R) or T / R lanes have the same, so the
+// link costs a wave once, not once a row.
+template <int OP, int FMT, int T, int R>
+__global__ __launch_bounds__(256, 2) void k_mx_rows_wave(MxRows a) {
+    static_assert(R <= T, "a lane ends with one row");
+    using W = typename Piece<FMT>::type;
+    constexpr int kTeams = 256 / T, kBytes = sizeof(W), kLead = T / R;
+    __shared__ double sh[kCols<OP> ? 4096 : 4];
+    __shared__ f64x2 vl[kDot<OP> ? 8 * T : 1];            // v's pairs, [pair][lane of the team]
+    const int tid = threadIdx.x, lane = tid & 63, tt = tid & (T - 1), team = tid / T;
+    const int nb = mx_blocks(a.D), pc = std::min(tt, 2 * nb - 1), own = tt / kLead;
+    const int64_t stride = (int64_t)gridDim.x * kTeams * R;
+    const unsigned vc = team * R * (unsigned)a.ldc + pc * kBytes, vs = team * R * (unsigned)a.lds + (pc >> 1);
+
+    double acc[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = 0.0;
+    if constexpr (kDot<OP>) {
+        for (int i = tid; i < 8 * T; i += 256) {
+            const int c = 16 * (i % T) + 2 * (i / T);
+            vl[i] = f64x2{c < a.D ? a.v[c] : 0.0, c + 1 < a.D ? a.v[c + 1] : 0.0};
+        }
+        __syncthreads();
+    }
+    double val = 0.0;
+    W next[R];
+    unsigned next_s[R];
+    RowScal next_r;
+    auto load = [&](int64_t n0) {
+        const MxRsrc rc = rows_rsrc(a.codes, n0, a.ldc, a.N, nb * (FMT == VT_MX_FP8 ? 32 : 16)), rs = rows_rsrc(a.scales, n0, a.lds, a.N, nb);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            next[r] = Piece<FMT>::load(rc, vc + r * (unsigned)a.ldc);
+            next_s[r] = __builtin_amdgcn_raw_buffer_load_b8(rs, vs + r * (unsigned)a.lds, 0, 0);
+        }
+        next_r = row_scal<OP>(a, std::min(n0 + team * R + own, a.N - 1));
+    };
+    int64_t n0 = (int64_t)blockIdx.x * kTeams * R;
+    load(n0);
+    const int64_t rounds = (a.N + stride - 1) / stride;
+    for (int64_t it = 0; it < rounds; ++it, n0 += stride) {
+        double x[R][16];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float s = mx_scale(next_s[r]);
+            each<8>([&](auto p) {
+                const f32x2 q = piece_pair<FMT, p>(next[r], s);
+                x[r][2 * p] = (double)q[0], x[r][2 * p + 1] = (double)q[1];
+            });
+        }
+        const RowScal scal = next_r;
+        load(n0 + stride);
+        double dot = 0.0;
+        if constexpr (kDot<OP>) {
+            double d[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) d[r] = 0.0;
+            asm volatile("" ::: "memory");       // v is read again every round: kept, it would take 32 registers
+            each<8>([&](auto p) {
+                const f64x2 vv = vl[p * T + tt];
+#pragma unroll
+                for (int r = 0; r < R; ++r) d[r] = fma(x[r][2 * p + 1], vv[1], fma(x[r][2 * p], vv[0], d[r]));
+            });
+            dot = team_sum<T, R>(d, lane);
+        }
+        const int64_t n = n0 + team * R + own;
+        double t = 0.0;
+        if (n < a.N) t = mx_row_op<OP>(a, n, scal, dot, tt % kLead == 0);
+        if constexpr (OP == OP_VALUE) val += tt % kLead == 0 ? t : 0.0;
+        if constexpr (kCols<OP>) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                double tr;
+                if constexpr (T == 64) tr = read_lane(t, r * kLead);
+                else tr = __shfl(t, (lane & ~(T - 1)) + r * kLead, 64);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[e] = fma(tr, x[r][e], acc[e]);
+            }
+        }
+    }
+    if constexpr (kCols<OP>) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sh[team * 16 * T + 16 * tt + e] = acc[e];
+        __syncthreads();
+        for (int c = tid; c < a.D; c += 256) {
+            double sum = 0.0;
+#pragma unroll
+            for (int g = 0; g < kTeams; ++g) sum += sh[g * 16 * T + c];
+            a.part[(int64_t)blockIdx.x * a.D + c] = sum;
+        }
+    }
+    if constexpr (OP == OP_VALUE) {
+        const double w = vt_sum64(val);
+        if (lane == 0) sh[tid >> 6] = w;
+        __syncthreads();
+        if (tid == 0) a.part[blockIdx.x] = sh[0] + sh[1] + sh[2] + sh[3];
+    }
+}
+
+// Wider rows: a workgroup of T threads a row, CPT pieces a thread, R rows a round; v in LDS (read once a round for all R
+// rows), the column sums in registers, one barrier a round for the dots.  v's pairs lie [piece / T][pair][piece % T] so
+// that the lanes of a read are next to each other.  KEEP: the round's numbers stay in registers as doubles (16 CPT R of
+// them) from the dot to the column sums; else the codes are decoded twice.
+template <int OP, int FMT, int T, int CPT, int R, bool KEEP>
+__global__ __launch_bounds__(T, 2) void k_mx_rows_wide(MxRows a) {
+    using W = typename Piece<FMT>::type;
+    constexpr int kBytes = sizeof(W), kWaves = T / 64, kLead = 64 / R;
+    static_assert(kWaves <= kLead, "a row's wave sums fit its lanes");
+    extern __shared__ __align__(16) double dyn[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int nb = mx_blocks(a.D), pieces = 2 * nb, own = lane / kLead;
+    f64x2* const vl = (f64x2*)dyn;
+    double* const red = dyn + (kDot<OP> ? 16 * pieces : 0);       // [2][R][kWaves]
+    const int last = pieces - (CPT - 1) * T;                      // pieces of the last round of threads, >= 1
+    unsigned vc[CPT], vs[CPT];
+    double acc[kCols<OP> ? CPT : 1][16];
+#pragma unroll
+    for (int k = 0; k < CPT; ++k) {
+        const int pc = std::min(tid + T * k, pieces - 1);
+        vc[k] = pc * kBytes, vs[k] = pc >> 1;
+        if constexpr (kCols<OP>) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[k][e] = 0.0;
+        }
+    }
+    if constexpr (kDot<OP>) {
+#pragma unroll
+        for (int k = 0; k < CPT; ++k) {
+            const int width = k < CPT - 1 ? T : last, c = 16 * (tid + T * k);
+            if (tid < width)
+#pragma unroll
+                for (int p = 0; p < 8; ++p)
+                    vl[8 * T * k + p * width + tid] = f64x2{c + 2 * p < a.D ? a.v[c + 2 * p] : 0.0, c + 2 * p + 1 < a.D ? a.v[c + 2 * p + 1] : 0.0};
+        }
+        __syncthreads();
+    }
+    double val = 0.0;
+    W next[R][CPT];
+    unsigned next_s[R][CPT];
+    RowScal next_r;
+    auto load = [&](int64_t n0) {
+        const MxRsrc rc = rows_rsrc(a.codes, n0, a.ldc, a.N, nb * (FMT == VT_MX_FP8 ? 32 : 16)), rs = rows_rsrc(a.scales, n0, a.lds, a.N, nb);
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int k = 0; k < CPT; ++k) {
+                next[r][k] = Piece<FMT>::load(rc, vc[k] + r * (unsigned)a.ldc);
+                next_s[r][k] = __builtin_amdgcn_raw_buffer_load_b8(rs, vs[k] + r * (unsigned)a.lds, 0, 0);
+            }
+        next_r = row_scal<OP>(a, std::min(n0 + own, a.N - 1));
+    };
+    const int64_t stride = (int64_t)gridDim.x * R, rounds = (a.N + stride - 1) / stride;
+    int64_t n0 = (int64_t)blockIdx.x * R;
+    load(n0);
+    for (int64_t it = 0; it < rounds; ++it, n0 += stride) {
+        W w[R][CPT];
+        float s[R][CPT];
+        double x[KEEP ? R : 1][KEEP ? CPT : 1][16];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int k = 0; k < CPT; ++k) {
+                w[r][k] = next[r][k], s[r][k] = mx_scale(next_s[r][k]);
+                if constexpr (KEEP)
+                    each<8>([&](auto p) {
+                        const f32x2 q = piece_pair<FMT, p>(w[r][k], s[r][k]);
+                        x[r][k][2 * p] = (double)q[0], x[r][k][2 * p + 1] = (double)q[1];
+                    });
+            }
+        const RowScal scal = next_r;
+        load(n0 + stride);
+        double dot = 0.0;
+        if constexpr (kDot<OP>) {
+            double d[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) d[r] = 0.0;
+#pragma unroll
+            for (int k = 0; k < CPT; ++k) {
+                const int width = k < CPT - 1 ? T : last;
+                if (k < CPT - 1 || tid < width)
+                    each<8>([&](auto p) {
+                        const f64x2 vv = vl[8 * T * k + p * width + tid];
+#pragma unroll
+                        for (int r = 0; r < R; ++r) {
+                            if constexpr (KEEP) {
+                                d[r] = fma(x[r][k][2 * p], vv[0], d[r]);
+                                d[r] = fma(x[r][k][2 * p + 1], vv[1], d[r]);
+                            } else {
+                                const f32x2 q = piece_pair<FMT, p>(w[r][k], s[r][k]);
+                                d[r] = fma((double)q[0], vv[0], d[r]);
+                                d[r] = fma((double)q[1], vv[1], d[r]);
+                            }
+                        }
+                    });
+            }
+            // this wave's sum of row `own`, then the waves' sums: every lane of the row's group adds them all
+            const double mine = team_sum<64, R>(d, lane);
+            double* const slot = red + (it & 1) * kWaves * R + own * kWaves;
+            if (lane % kLead == 0) slot[wave] = mine;
+            vt_lds_barrier();
+            const double part[1] = {slot[lane & (kWaves - 1)]};
+            dot = team_sum<kWaves, 1>(part, lane);
+        }
+        const int64_t n = n0 + own;
+        double t = 0.0;
+        if (n < a.N) t = mx_row_op<OP>(a, n, scal, dot, wave == 0 && lane % kLead == 0);
+        if constexpr (OP == OP_VALUE) val += wave == 0 && lane % kLead == 0 ? t : 0.0;
+        if constexpr (kCols<OP>) {
+            double tr[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) tr[r] = read_lane(t, r * kLead);
+            if constexpr (kDot<OP> && !KEEP) {
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int k = 0; k < CPT; ++k) decode_again(w[r][k], s[r][k]);
+            }
+#pragma unroll
+            for (int k = 0; k < CPT; ++k)
+                if (k < CPT - 1 || tid < last)
+                    each<8>([&](auto p) {
+#pragma unroll
+                        for (int r = 0; r < R; ++r) {
+                            double x0, x1;
+                            if constexpr (KEEP) {
+                                x0 = x[r][k][2 * p], x1 = x[r][k][2 * p + 1];
+                            } else {
+                                const f32x2 q = piece_pair<FMT, p>(w[r][k], s[r][k]);
+                                x0 = (double)q[0], x1 = (double)q[1];
+                            }
+                            acc[k][2 * p] = fma(tr[r], x0, acc[k][2 * p]);
+                            acc[k][2 * p + 1] = fma(tr[r], x1, acc[k][2 * p + 1]);
+                        }
+                    });
+        }
+    }
+    if constexpr (kCols<OP>) {
+        double* out = a.part + (int64_t)blockIdx.x * a.D;
+#pragma unroll
+        for (int k = 0; k < CPT; ++k)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int c = 16 * (tid + T * k) + e;
+                if (c < a.D) out[c] = acc[k][e];
+            }
+    }
+    if constexpr (OP == OP_VALUE) {
+        if (wave == 0) {
+            val = vt_sum64(val);
+            if (lane == 0) a.part[blockIdx.x] = val;
+        }
+    }
+}
+
+// ---- two passes: rows too wide for one workgroup's registers and LDS ----------------------------------------------------
+// One wave per row takes the dots and leaves t_n in the workspace; then every thread owns eight columns and walks a slab.
 
 // Eight values of a row, columns 8 g .. 8 g + 7.
 template <int FMT>
@@ -81,7 +474,7 @@ __global__ __launch_bounds__(256) void k_mx_dots(MxRows a) {
             dot = vt_sum64(dot);
         }
         if (lane == 0) {
-            const double t = mx_row_op<OP>(a, n, dot);
+            const double t = mx_row_op<OP>(a, n, row_scal<OP>(a, n), dot, true);
             if (a.t) a.t[n] = t;
         }
     }
@@ -140,23 +533,95 @@ __global__ __launch_bounds__(1024) void k_mx_sum(const double* t, int64_t N, dou
     }
 }
 
+// Which kernel takes a width: 2, 8, 32 or 64 lanes of a wave (D <= 1024), a workgroup of 128, 256 or 512 threads with one
+// piece each (D <= 8192: fewer threads with more pieces were slower, D = 4096: 112 us in 256 x 1, 143 in 128 x 2), 512 with
+// two or three, else two passes.  v and the sums of a round share 160 KB of LDS: D <= 20352 in one pass.
+constexpr int kOnePassPieces = (160 * 1024 - 1024) / 128;
+
+struct RowsPlan {
+    int lanes, threads, cpt;      // lanes > 0: wave kernel; else threads > 0: wide kernel
+    int grid;                     // = slabs of partial sums
+};
+
+// Rows a round.  One piece a thread: 4, kept as doubles (128 registers).  Two pieces: 4, decoded twice (N = 50 000,
+// D = 16 384: 206 us; 2 kept rows 222).  Three pieces: 4 fit for E2M1; for E4M3 2 (N = 100 000, D = 20 000: 503 us; 4 spill:
+// 985).
+constexpr int wave_rows(int lanes) { return lanes < 4 ? lanes : 4; }
+constexpr int wide_rows(int cpt, int format) { return cpt == 3 && format == VT_MX_FP8 ? 2 : 4; }
+
 int col_tiles(int D) { return (D + 2047) / 2048; }
-int64_t slabs(int64_t N, int D) { return std::max<int64_t>(1, std::min<int64_t>(N, std::max(1, 4 * vt_num_cu() / col_tiles(D)))); }
+
+RowsPlan rows_plan(int format, int64_t N, int D, int64_t ldc, int64_t lds) {
+    const int pieces = 2 * mx_blocks(D), cu = vt_num_cu();
+    RowsPlan p{0, 0, 0, 0};
+    int64_t rounds;               // of all workgroups together
+    int most;                     // workgroups that are resident together
+    // (offsets inside a round are 32 bits: 256 rows at most)
+    const bool far = ldc >= 1 << 22 || lds >= 1 << 22;
+    if (pieces <= 64 && !far) {
+        p.lanes = pieces <= 2 ? 2 : pieces <= 8 ? 8 : pieces <= 32 ? 32 : 64;
+        const int rows = 256 / p.lanes * wave_rows(p.lanes);
+        rounds = (N + rows - 1) / rows, most = 2 * cu;
+    } else if (pieces <= kOnePassPieces && !far) {
+        p.threads = pieces <= 128 ? 128 : pieces <= 256 ? 256 : 512;
+        p.cpt = (pieces + p.threads - 1) / p.threads;
+        const int rows = wide_rows(p.cpt, format);
+        rounds = (N + rows - 1) / rows;
+        most = cu * std::max(1, std::min(512 / p.threads, (160 * 1024) / (128 * pieces + 1024)));
+    } else {
+        p.grid = (int)std::max<int64_t>(1, std::min<int64_t>(N, std::max(1, 4 * cu / col_tiles(D))));
+        return p;
+    }
+    // the same number of rounds for every workgroup
+    const int64_t each = std::max<int64_t>(1, (rounds + most - 1) / most);
+    p.grid = (int)std::max<int64_t>(1, (rounds + each - 1) / each);
+    return p;
+}
+
+template <int OP, int FMT, int T>
+void launch_wave(const MxRows& a, int grid, hipStream_t st) {
+    hipLaunchKernelGGL((k_mx_rows_wave<OP, FMT, T, wave_rows(T)>), dim3(grid), dim3(256), 0, st, a);
+}
+
+template <int OP, int FMT, int T, int CPT>
+int launch_wide(const MxRows& a, int grid, hipStream_t st) {
+    constexpr bool keep = CPT == 1;
+    constexpr int R = wide_rows(CPT, FMT);
+    const size_t lds = (kDot<OP> ? 128 * (size_t)(2 * mx_blocks(a.D)) : 0) + 2 * (T / 64) * R * sizeof(double);
+    static VtLdsAttr attr;
+    if (vt_allow_big_lds((const void*)k_mx_rows_wide<OP, FMT, T, CPT, R, keep>, attr, 160 * 1024) != VT_OK) return VT_ERR_HIP;
+    hipLaunchKernelGGL((k_mx_rows_wide<OP, FMT, T, CPT, R, keep>), dim3(grid), dim3(T), lds, st, a);
+    return VT_OK;
+}
 
 template <int OP, int FMT>
-int run(MxRows a, int* nslabs, hipStream_t st) {
+int run(MxRows a, const RowsPlan& p, hipStream_t st) {
+    if (p.lanes > 0) {
+        switch (p.lanes) {
+            case 2: launch_wave<OP, FMT, 2>(a, p.grid, st); break;
+            case 8: launch_wave<OP, FMT, 8>(a, p.grid, st); break;
+            case 32: launch_wave<OP, FMT, 32>(a, p.grid, st); break;
+            default: launch_wave<OP, FMT, 64>(a, p.grid, st); break;
+        }
+        return vt_launch_status();
+    }
+    if (p.threads > 0) {
+        const int rc = p.threads == 128   ? launch_wide<OP, FMT, 128, 1>(a, p.grid, st)
+                       : p.threads == 256 ? launch_wide<OP, FMT, 256, 1>(a, p.grid, st)
+                       : p.cpt == 1       ? launch_wide<OP, FMT, 512, 1>(a, p.grid, st)
+                       : p.cpt == 2       ? launch_wide<OP, FMT, 512, 2>(a, p.grid, st)
+                                          : launch_wide<OP, FMT, 512, 3>(a, p.grid, st);
+        return rc != VT_OK ? rc : vt_launch_status();
+    }
     const int grid = (int)std::min<int64_t>((a.N + 3) / 4, 8 * (int64_t)vt_num_cu());
     hipLaunchKernelGGL((k_mx_dots<OP, FMT>), dim3(grid), dim3(256), 0, st, a);
-    if constexpr (kCols<OP>) {
-        *nslabs = (int)slabs(a.N, a.D);
-        hipLaunchKernelGGL((k_mx_columns<FMT>), dim3(col_tiles(a.D), *nslabs), dim3(256), 0, st, a);
-    }
+    if constexpr (kCols<OP>) hipLaunchKernelGGL((k_mx_columns<FMT>), dim3(col_tiles(a.D), p.grid), dim3(256), 0, st, a);
     return vt_launch_status();
 }
 
 template <int OP>
-int run(int format, MxRows a, int* nslabs, hipStream_t st) {
-    return format == VT_MX_FP8 ? run<OP, VT_MX_FP8>(a, nslabs, st) : run<OP, VT_MX_FP4>(a, nslabs, st);
+int run(int format, const MxRows& a, const RowsPlan& p, hipStream_t st) {
+    return format == VT_MX_FP8 ? run<OP, VT_MX_FP8>(a, p, st) : run<OP, VT_MX_FP4>(a, p, st);
 }
 
 int finalize(const double* part, int P, int D, const double* beta, const double* bvec, double beta_scalar, double* out,
@@ -165,13 +630,20 @@ int finalize(const double* part, int P, int D, const double* beta, const double*
     return vt_launch_status();
 }
 
-MxRows rows_of(const void* codes, int64_t ldc, const void* scales, int64_t lds, int64_t N, int D, void* ws) {
+// Workspace: slabs of partial column sums (VALUE: one number a workgroup, or a row), and t for the two passes.
+// Enough for both formats and any strides.
+size_t ws_doubles(int64_t N, int D) {
+    const int g = std::max(rows_plan(VT_MX_FP8, N, D, 0, 0).grid, rows_plan(VT_MX_FP4, N, D, 0, 0).grid);
+    return std::max((size_t)g * D, (size_t)rows_plan(VT_MX_FP8, N, D, 1 << 30, 0).grid * D + (size_t)N);
+}
+
+MxRows rows_of(const void* codes, int64_t ldc, const void* scales, int64_t lds, int64_t N, int D, void* ws, const RowsPlan& p) {
     MxRows a{};
     a.codes = (const uint8_t*)codes;
     a.scales = (const uint8_t*)scales;
     a.ldc = ldc, a.lds = lds, a.N = N, a.D = D;
     a.part = (double*)ws;
-    a.t = a.part + slabs(N, D) * D;
+    a.t = a.part + (size_t)p.grid * D;
     return a;
 }
 
@@ -179,14 +651,15 @@ MxRows rows_of(const void* codes, int64_t ldc, const void* scales, int64_t lds, 
 
 extern "C" size_t vt_mx_rows_workspace_bytes(int64_t N, int D) {
     if (N < 0 || D < 1) return 0;
-    return ((size_t)slabs(N, D) * D + (size_t)N) * sizeof(double);
+    return ws_doubles(N, D) * sizeof(double);
 }
 
 #define VT_MX_ROWS_PROLOGUE                                                                  \
     if (!mx_rows_ok(format, codes, ldc, scales, lds, N, D)) return VT_ERR_BAD_ARG;           \
     if (!ws || ws_bytes < vt_mx_rows_workspace_bytes(N, D)) return VT_ERR_WORKSPACE;         \
     hipStream_t st = (hipStream_t)stream;                                                    \
-    MxRows a = rows_of(codes, ldc, scales, lds, N, D, ws);
+    const RowsPlan p = rows_plan(format, N, D, ldc, lds);                                        \
+    MxRows a = rows_of(codes, ldc, scales, lds, N, D, ws, p);
 
 extern "C" int vt_mx_glm_link(int family, int format, const void* codes, int64_t ldc, const void* scales, int64_t lds,
                               const double* theta, const double* y, const double* w, const double* offset, double scale,
@@ -197,7 +670,7 @@ extern "C" int vt_mx_glm_link(int family, int format, const void* codes, int64_t
     if (!theta || !y || !w) return VT_ERR_BAD_ARG;
     a.v = theta, a.y = y, a.w = w, a.offset = offset, a.scale = scale, a.family = family;
     a.z = z, a.r = r, a.d = d, a.t = nullptr;
-    return run<OP_LINK>(format, a, nullptr, st);
+    return run<OP_LINK>(format, a, p, st);
 }
 
 extern "C" int vt_mx_glm_grad(int family, int format, const void* codes, int64_t ldc, const void* scales, int64_t lds,
@@ -207,10 +680,9 @@ extern "C" int vt_mx_glm_grad(int family, int format, const void* codes, int64_t
     VT_MX_ROWS_PROLOGUE
     if (family < 0 || family > 2 || !theta || !g || (N > 0 && (!y || !w))) return VT_ERR_BAD_ARG;
     a.v = theta, a.y = y, a.w = w, a.offset = offset, a.scale = scale, a.family = family, a.r = r, a.d = d;
-    int P = 0;
     if (N > 0)
-        if (int rc = run<OP_GRAD>(format, a, &P, st)) return rc;
-    return finalize(a.part, P, D, prior, prior ? theta : nullptr, 0.0, g, st);
+        if (int rc = run<OP_GRAD>(format, a, p, st)) return rc;
+    return finalize(a.part, N > 0 ? p.grid : 0, D, prior, prior ? theta : nullptr, 0.0, g, st);
 }
 
 extern "C" int vt_mx_glm_value(int family, int format, const void* codes, int64_t ldc, const void* scales, int64_t lds,
@@ -220,8 +692,9 @@ extern "C" int vt_mx_glm_value(int family, int format, const void* codes, int64_
     if (family < 0 || family > 2 || !theta || !value || (N > 0 && (!y || !w))) return VT_ERR_BAD_ARG;
     a.v = theta, a.y = y, a.w = w, a.offset = offset, a.family = family;
     if (N > 0)
-        if (int rc = run<OP_VALUE>(format, a, nullptr, st)) return rc;
-    hipLaunchKernelGGL(k_mx_sum, dim3(1), dim3(1024), 0, st, a.t, N, scale, value);
+        if (int rc = run<OP_VALUE>(format, a, p, st)) return rc;
+    const bool one_pass = p.lanes > 0 || p.threads > 0;
+    hipLaunchKernelGGL(k_mx_sum, dim3(1), dim3(1024), 0, st, one_pass ? a.part : a.t, one_pass && N > 0 ? p.grid : N, scale, value);
     return vt_launch_status();
 }
 
@@ -231,10 +704,9 @@ extern "C" int vt_mx_glm_hvp(int format, const void* codes, int64_t ldc, const v
     VT_MX_ROWS_PROLOGUE
     if (!v || !out || (N > 0 && !d)) return VT_ERR_BAD_ARG;
     a.v = v, a.y = d;
-    int P = 0;
     if (N > 0)
-        if (int rc = run<OP_HVP>(format, a, &P, st)) return rc;
-    return finalize(a.part, P, D, prior, prior || prior_scalar != 0.0 ? v : nullptr, prior_scalar, out, st);
+        if (int rc = run<OP_HVP>(format, a, p, st)) return rc;
+    return finalize(a.part, N > 0 ? p.grid : 0, D, prior, prior || prior_scalar != 0.0 ? v : nullptr, prior_scalar, out, st);
 }
 
 extern "C" int vt_mx_gemv(int format, const void* codes, int64_t ldc, const void* scales, int64_t lds, const double* v,
@@ -243,7 +715,7 @@ extern "C" int vt_mx_gemv(int format, const void* codes, int64_t ldc, const void
     if (N == 0) return VT_OK;
     if (!v || !out) return VT_ERR_BAD_ARG;
     a.v = v, a.z = out, a.t = nullptr;
-    return run<OP_GEMV>(format, a, nullptr, st);
+    return run<OP_GEMV>(format, a, p, st);
 }
 
 extern "C" int vt_mx_gemv_t(int format, const void* codes, int64_t ldc, const void* scales, int64_t lds, const double* u1,
@@ -251,8 +723,7 @@ extern "C" int vt_mx_gemv_t(int format, const void* codes, int64_t ldc, const vo
     VT_MX_ROWS_PROLOGUE
     if (!out || (N > 0 && !u1)) return VT_ERR_BAD_ARG;
     a.y = u1, a.w = u2;
-    int P = 0;
     if (N > 0)
-        if (int rc = run<OP_GEMVT>(format, a, &P, st)) return rc;
-    return finalize(a.part, P, D, nullptr, nullptr, 0.0, out, st);
+        if (int rc = run<OP_GEMVT>(format, a, p, st)) return rc;
+    return finalize(a.part, N > 0 ? p.grid : 0, D, nullptr, nullptr, 0.0, out, st);
 }
