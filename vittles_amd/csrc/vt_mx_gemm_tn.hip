@@ -22,7 +22,6 @@ struct MxTN {
     int Da, Db;
     const void* B;
     int64_t ldb;
-    bool vec;                       // B's rows are 16-byte aligned
     const double* rowscale;
     float alpha;
     const float* bias;
@@ -31,15 +30,16 @@ struct MxTN {
     float* part;                    // [slabs][Da][Db], when there are several
 };
 
-// A workgroup of WM x WN waves, each MT x NT products of 32 x 32; kRows rows a chunk, two chunks in LDS.
+// A workgroup of WM x WN waves, each MT x NT products of 32 x 32; kRows rows a chunk, two chunks in LDS (64 rows, where
+// they fit, halve the barriers: 16384 x 4096 x 1000 in bfloat16 165 -> 151 us).
 template <int MT, int NT, int WM, int WN, int PARTS>
 struct TnShape {
-    static constexpr int kThreads = 64 * WM * WN, BM = 32 * MT * WM, BN = 32 * NT * WN, kRows = 32;
+    static constexpr int kThreads = 64 * WM * WN, BM = 32 * MT * WM, BN = 32 * NT * WN, kRows = PARTS == 1 && BN == 256 ? 64 : 32;
     // 64 bytes behind every row: the four rows of a transposing read lie in different banks
     static constexpr int kPitchA = 2 * BM + 64, kPitchB = 2 * BN + 64;
     static constexpr int kA = kRows * kPitchA, kB = kRows * kPitchB, kBuf = kA + PARTS * kB, kLds = 2 * kBuf;
-    static constexpr int kLoadsA = kRows * BM / 8 / kThreads, kLoadsB = kRows * BN / 8 / kThreads;      // 8 columns each
-    static_assert(kRows * BM / 8 % kThreads == 0 && kRows * BN / 8 % kThreads == 0, "even shares");
+    static constexpr int kLoadsA = kRows * BM / 16 / kThreads, kLoadsB = kRows * BN / 8 / kThreads;      // 16 and 8 columns each
+    static_assert(kRows * BM / 16 % kThreads == 0 && kRows * BN / 8 % kThreads == 0, "even shares");
 };
 
 template <typename T, bool SCALED> constexpr int kParts = SCALED || std::is_same<T, float>::value ? 3 : std::is_same<T, f16>::value ? 2 : 1;
@@ -67,90 +67,131 @@ __device__ __forceinline__ s16x8 read_tr(const uint8_t* p, int next4) {
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-template <int FMT, typename T, bool SCALED, int MT, int NT, int WM, int WN, bool SPLIT>
-__global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tn(MxTN a) {
+// A descriptor that ends `bytes` behind p; loads past it give 0.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tn_rsrc(const void* base, int64_t bytes) {
+    const uint64_t p = (uint64_t)base;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)p), hi = __builtin_amdgcn_readfirstlane((uint32_t)(p >> 32));
+    const uint32_t n = bytes <= 0 ? 0 : (uint32_t)std::min<int64_t>(bytes, 0x7fffffff);
+    return __builtin_amdgcn_make_buffer_rsrc((void*)(((uint64_t)hi << 32) | lo), 0, __builtin_amdgcn_readfirstlane(n), 0x00020000);
+}
+constexpr unsigned kNowhere = 0x80000000u;       // an offset past every descriptor
+
+template <int FMT, typename T, bool SCALED, int MT, int NT, int WM, int WN, bool VEC, bool SPLIT>
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tn(MxTN a, int tiles_d, int tiles_k) {
     constexpr int PARTS = kParts<T, SCALED>;
     using S = TnShape<MT, NT, WM, WN, PARTS>;
+    using W = typename std::conditional<FMT == VT_MX_FP8, u32x4, u32x2>::type;      // 16 codes
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WN, wn = wave % WN;
-    const int d0 = blockIdx.x * S::BM, k0 = blockIdx.y * S::BN;
-    const int64_t n_lo = (int64_t)blockIdx.z * a.rows, n_hi = std::min(a.N, n_lo + a.rows);
+    // workgroups go to the 8 XCDs in turn: each gets a run of tiles, slab by slab, which share the slab's rows in its L2
+    const int tiles = tiles_d * tiles_k, per_xcd = gridDim.x >> 3;
+    const int t = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3), slab = t / tiles, tile = t - slab * tiles;
+    const int64_t n_lo = slab * a.rows, n_hi = std::min(a.N, n_lo + a.rows);
+    if (slab * a.rows >= std::max<int64_t>(a.N, 1)) return;
+    const int d0 = tile / tiles_k * S::BM, k0 = tile % tiles_k * S::BN;
     const int width = mx_blocks(a.Da) * kMxBlock;
 
-    u32x2 ca[S::kLoadsA];
-    unsigned sc[S::kLoadsA];
-    T cb[S::kLoadsB][8];
-    double rs[S::kLoadsB];
-    auto fetch = [&](int64_t n0) {
+    unsigned va[S::kLoadsA], vs[S::kLoadsA], vb[S::kLoadsB];
+#pragma unroll
+    for (int i = 0; i < S::kLoadsA; ++i) {
+        const int e = tid + S::kThreads * i, c = d0 + e % (S::BM / 16) * 16;
+        const unsigned r = e / (S::BM / 16);
+        va[i] = c < width ? r * (unsigned)a.ldc + (FMT == VT_MX_FP8 ? c : c / 2) : kNowhere;
+        vs[i] = c < width ? r * (unsigned)a.lds + c / kMxBlock : kNowhere;
+    }
+#pragma unroll
+    for (int i = 0; i < S::kLoadsB; ++i) {
+        const int e = tid + S::kThreads * i, c = k0 + e % (S::BN / 8) * 8;
+        vb[i] = c < a.Db ? (e / (S::BN / 8) * (unsigned)a.ldb + c) * (unsigned)sizeof(T) : kNowhere;
+    }
+    struct Chunk {
+        W ca[S::kLoadsA];
+        unsigned sc[S::kLoadsA];
+        u32x4 cb[S::kLoadsB][sizeof(T) / 2];
+        double rs[SCALED ? S::kLoadsB : 1];
+    };
+    // rows behind the slab's end come as 0; columns of a piece behind the last one are the next row's and end in columns
+    // of the tile that are not stored
+    auto fetch = [&](int64_t n0, Chunk& x) {
+        const int64_t left = n_hi - n0;
+        const auto ra = tn_rsrc(a.codes + n0 * a.ldc, left > 0 ? (left - 1) * a.ldc + (FMT == VT_MX_FP8 ? width : width / 2) : 0);
+        const auto rs = tn_rsrc(a.scales + n0 * a.lds, left > 0 ? (left - 1) * a.lds + width / kMxBlock : 0);
+        const int64_t last = VEC ? (a.Db + 7) / 8 * 8 : a.Db;
+        const auto rb = tn_rsrc((const T*)a.B + n0 * a.ldb, left > 0 ? ((left - 1) * a.ldb + last) * (int64_t)sizeof(T) : 0);
 #pragma unroll
         for (int i = 0; i < S::kLoadsA; ++i) {
-            const int e = tid + S::kThreads * i, c = d0 + e % (S::BM / 8) * 8;
-            const int64_t n = n0 + e / (S::BM / 8);
-            ca[i] = u32x2{0, 0};
-            sc[i] = 127;
-            if (n < n_hi && c < width) {
-                if constexpr (FMT == VT_MX_FP8) ca[i] = *(const u32x2*)(a.codes + n * a.ldc + c);
-                else ca[i][0] = *(const unsigned*)(a.codes + n * a.ldc + c / 2);
-                sc[i] = a.scales[n * a.lds + c / kMxBlock];
-            }
+            if constexpr (FMT == VT_MX_FP8) x.ca[i] = __builtin_bit_cast(W, __builtin_amdgcn_raw_buffer_load_b128(ra, va[i], 0, 0));
+            else x.ca[i] = __builtin_bit_cast(W, __builtin_amdgcn_raw_buffer_load_b64(ra, va[i], 0, 0));
+            x.sc[i] = __builtin_amdgcn_raw_buffer_load_b8(rs, vs[i], 0, 0);
         }
 #pragma unroll
         for (int i = 0; i < S::kLoadsB; ++i) {
-            const int e = tid + S::kThreads * i, c = k0 + e % (S::BN / 8) * 8;
-            const int64_t n = n0 + e / (S::BN / 8);
-            const T* p = (const T*)a.B + n * a.ldb + c;
-            if (n < n_hi && a.vec && c + 8 <= a.Db) {
-                constexpr int W = (int)sizeof(T) / 2;
-                u32x4 t[W];
+            if constexpr (VEC) {
 #pragma unroll
-                for (int j = 0; j < W; ++j) t[j] = ((const u32x4*)p)[j];
-                __builtin_memcpy(cb[i], t, sizeof(t));
+                for (int j = 0; j < (int)sizeof(T) / 2; ++j)
+                    x.cb[i][j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rb, vb[i] + 16 * j, 0, 0));
             } else {
+                T v[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) cb[i][j] = n < n_hi && c + j < a.Db ? p[j] : (T)0.0f;
+                for (int j = 0; j < 8; ++j) {
+                    if constexpr (sizeof(T) == 4) v[j] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(rb, vb[i] + 4 * j, 0, 0));
+                    else v[j] = __builtin_bit_cast(T, (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(rb, vb[i] + 2 * j, 0, 0));
+                }
+                __builtin_memcpy(x.cb[i], v, sizeof(v));
             }
-            if constexpr (SCALED) rs[i] = n < n_hi ? a.rowscale[n] : 0.0;
+            if constexpr (SCALED) {
+                const int64_t n = n0 + (tid + S::kThreads * i) / (S::BN / 8);
+                x.rs[i] = n < n_hi ? a.rowscale[n] : 0.0;
+            }
         }
     };
-    auto put = [&](uint8_t* base) {
+    auto put = [&](const Chunk& x, uint8_t* base) {
 #pragma unroll
         for (int i = 0; i < S::kLoadsA; ++i) {
             const int e = tid + S::kThreads * i;
-            const float s = mx_scale(sc[i]);
-            bf16x2 v[4];
-            if constexpr (FMT == VT_MX_FP8) {
-                v[0] = mx_pair_bf16<FMT, 0>(ca[i][0], s), v[1] = mx_pair_bf16<FMT, 1>(ca[i][0], s);
-                v[2] = mx_pair_bf16<FMT, 0>(ca[i][1], s), v[3] = mx_pair_bf16<FMT, 1>(ca[i][1], s);
-            } else {
-                v[0] = mx_pair_bf16<FMT, 0>(ca[i][0], s), v[1] = mx_pair_bf16<FMT, 1>(ca[i][0], s);
-                v[2] = mx_pair_bf16<FMT, 2>(ca[i][0], s), v[3] = mx_pair_bf16<FMT, 3>(ca[i][0], s);
+            const float s = mx_scale(x.sc[i]);
+            u32x4 v[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                bf16x2 q[4];
+                if constexpr (FMT == VT_MX_FP8) {
+                    q[0] = mx_pair_bf16<FMT, 0>(x.ca[i][2 * h], s), q[1] = mx_pair_bf16<FMT, 1>(x.ca[i][2 * h], s);
+                    q[2] = mx_pair_bf16<FMT, 0>(x.ca[i][2 * h + 1], s), q[3] = mx_pair_bf16<FMT, 1>(x.ca[i][2 * h + 1], s);
+                } else {
+                    q[0] = mx_pair_bf16<FMT, 0>(x.ca[i][h], s), q[1] = mx_pair_bf16<FMT, 1>(x.ca[i][h], s);
+                    q[2] = mx_pair_bf16<FMT, 2>(x.ca[i][h], s), q[3] = mx_pair_bf16<FMT, 3>(x.ca[i][h], s);
+                }
+                v[h] = u32x4{__builtin_bit_cast(unsigned, q[0]), __builtin_bit_cast(unsigned, q[1]), __builtin_bit_cast(unsigned, q[2]),
+                             __builtin_bit_cast(unsigned, q[3])};
             }
-            *(u32x4*)(base + e / (S::BM / 8) * S::kPitchA + e % (S::BM / 8) * 16) =
-                u32x4{__builtin_bit_cast(unsigned, v[0]), __builtin_bit_cast(unsigned, v[1]), __builtin_bit_cast(unsigned, v[2]),
-                      __builtin_bit_cast(unsigned, v[3])};
+            // eight lanes write the first halves of their 32 bytes while the next eight write the second: all banks
+            uint8_t* p = base + e / (S::BM / 16) * S::kPitchA + e % (S::BM / 16) * 32;
+            const bool odd = lane & 8;
+            *(u32x4*)(p + (odd ? 16 : 0)) = odd ? v[1] : v[0];
+            *(u32x4*)(p + (odd ? 0 : 16)) = odd ? v[0] : v[1];
         }
 #pragma unroll
         for (int i = 0; i < S::kLoadsB; ++i) {
             const int e = tid + S::kThreads * i;
             uint8_t* p = base + S::kA + e / (S::BN / 8) * S::kPitchB + e % (S::BN / 8) * 16;
             if constexpr (PARTS == 1) {
-                u32x4 t;
-                __builtin_memcpy(&t, cb[i], 16);
-                *(u32x4*)p = t;
+                *(u32x4*)p = x.cb[i][0];
             } else {
+                T c[8];
+                __builtin_memcpy(c, x.cb[i], sizeof(c));
                 u32x4 w[PARTS];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    unsigned x[2][PARTS];
+                    unsigned y[2][PARTS];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        float b = (float)cb[i][2 * j + h];
-                        if constexpr (SCALED) b = (float)(rs[i] * (double)b);
-                        split<PARTS>(b, x[h]);
+                        float b = (float)c[2 * j + h];
+                        if constexpr (SCALED) b = (float)(x.rs[i] * (double)b);
+                        split<PARTS>(b, y[h]);
                     }
 #pragma unroll
-                    for (int q = 0; q < PARTS; ++q) w[q][j] = x[0][q] | x[1][q] << 16;
+                    for (int q = 0; q < PARTS; ++q) w[q][j] = y[0][q] | y[1][q] << 16;
                 }
 #pragma unroll
                 for (int q = 0; q < PARTS; ++q) *(u32x4*)(p + q * S::kB) = w[q];
@@ -190,17 +231,20 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tn(MxTN a) {
         }
     };
 
-    int buf = 0;
-    if (n_lo < n_hi) {
-        fetch(n_lo);
-        put(lds);
-    }
-    for (int64_t n0 = n_lo; n0 < n_hi; n0 += S::kRows, buf ^= 1) {
-        const bool more = n0 + S::kRows < n_hi;
+    // two chunks ahead in registers, one in LDS; chunks behind the end are zeros and add nothing
+    Chunk even, odd;
+    fetch(n_lo, even);
+    fetch(n_lo + S::kRows, odd);
+    put(even, lds);
+    for (int64_t n0 = n_lo; n0 < n_hi; n0 += 2 * S::kRows) {
         vt_lds_barrier();           // the chunk is written, and the other place is read
-        if (more) fetch(n0 + S::kRows);
-        multiply(lds + buf * S::kBuf);
-        if (more) put(lds + (buf ^ 1) * S::kBuf);
+        fetch(n0 + 2 * S::kRows, even);
+        multiply(lds);
+        put(odd, lds + S::kBuf);
+        vt_lds_barrier();
+        fetch(n0 + 3 * S::kRows, odd);
+        multiply(lds + S::kBuf);
+        put(even, lds);
     }
 
     // lane, element e of a 32 x 32 result: row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32
@@ -215,7 +259,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tn(MxTN a) {
                 for (int e = 0; e < 16; ++e) {
                     const int d = d0 + 32 * (wm * MT + i) + 8 * (e / 4) + 4 * h + e % 4;
                     if (d < a.Da) {
-                        if constexpr (SPLIT) a.part[((int64_t)blockIdx.z * a.Da + d) * a.Db + k] = acc[i][j][e];
+                        if constexpr (SPLIT) a.part[((int64_t)slab * a.Da + d) * a.Db + k] = acc[i][j][e];
                         else a.C[(int64_t)d * a.ldo + k] = a.alpha * acc[i][j][e] + (a.bias ? a.bias[k] : 0.0f);
                     }
                 }
@@ -223,7 +267,28 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tn(MxTN a) {
         }
 }
 
-__global__ __launch_bounds__(256) void k_mx_tn_join(MxTN a, int slabs) {
+// The slabs' sums in a fixed order: 32 elements a workgroup, G groups of threads that each take every G-th slab.
+template <int G>
+__global__ __launch_bounds__(32 * G) void k_mx_tn_join(MxTN a, int slabs) {
+    __shared__ float sh[G][33];
+    const int x = threadIdx.x & 31, g = threadIdx.x >> 5;
+    const int64_t total = (int64_t)a.Da * a.Db, i = (int64_t)blockIdx.x * 32 + x;
+    float s = 0.0f;
+    if (i < total)
+        for (int p = g; p < slabs; p += G) s += a.part[p * total + i];
+    sh[g][x] = s;
+    __syncthreads();
+    if (g == 0 && i < total) {
+#pragma unroll
+        for (int q = 1; q < G; ++q) s += sh[q][x];
+        const int64_t d = i / a.Db;
+        const int k = (int)(i - d * a.Db);
+        a.C[d * a.ldo + k] = a.alpha * s + (a.bias ? a.bias[k] : 0.0f);
+    }
+}
+
+// The same for few slabs: a thread an element.
+__global__ __launch_bounds__(256) void k_mx_tn_join_few(MxTN a, int slabs) {
     const int64_t total = (int64_t)a.Da * a.Db;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
         float s = 0.0f;
@@ -241,36 +306,44 @@ struct TnPlan {
 
 TnPlan plan(int64_t N, int Da, int Db) {
     TnPlan p;
-    if (Db > 64) p.bm = 256, p.bn = 128;
+    if (Db > 128) p.bm = 256, p.bn = 256;
+    else if (Db > 64) p.bm = 256, p.bn = 128;
     else p.bm = 128, p.bn = 64;
     const int64_t tiles = (int64_t)((Da + p.bm - 1) / p.bm) * ((Db + p.bn - 1) / p.bn);
-    const int64_t want = std::max<int64_t>(1, 2 * vt_num_cu() / tiles), most = std::max<int64_t>(1, N / 128);
+    const int64_t want = std::max<int64_t>(1, (p.bn == 256 ? 1 : 2) * vt_num_cu() / tiles), most = std::max<int64_t>(1, N / 128);
     p.slabs = (int)std::min(want, most);
-    p.rows = (std::max<int64_t>(1, (N + p.slabs - 1) / p.slabs) + 31) / 32 * 32;
+    p.rows = (std::max<int64_t>(1, (N + p.slabs - 1) / p.slabs) + 127) / 128 * 128;
     p.slabs = (int)std::max<int64_t>(1, (N + p.rows - 1) / p.rows);
     return p;
 }
 
-template <int FMT, typename T, bool SCALED, int MT, int NT, int WM, int WN>
+template <int FMT, typename T, bool SCALED, int MT, int NT, int WM, int WN, bool VEC>
 int launch(const MxTN& a, const TnPlan& p, hipStream_t st) {
     using S = TnShape<MT, NT, WM, WN, kParts<T, SCALED>>;
-    const dim3 grid((a.Da + S::BM - 1) / S::BM, (a.Db + S::BN - 1) / S::BN, p.slabs);
+    const int td = (a.Da + S::BM - 1) / S::BM, tk = (a.Db + S::BN - 1) / S::BN;
+    const dim3 grid((unsigned)(((int64_t)td * tk * p.slabs + 7) / 8 * 8));
     static VtLdsAttr attr_split, attr_whole;
     if (p.slabs > 1) {
-        if (vt_allow_big_lds((const void*)k_mx_tn<FMT, T, SCALED, MT, NT, WM, WN, true>, attr_split, S::kLds) != VT_OK) return VT_ERR_HIP;
-        hipLaunchKernelGGL((k_mx_tn<FMT, T, SCALED, MT, NT, WM, WN, true>), grid, dim3(S::kThreads), S::kLds, st, a);
+        if (vt_allow_big_lds((const void*)k_mx_tn<FMT, T, SCALED, MT, NT, WM, WN, VEC, true>, attr_split, S::kLds) != VT_OK) return VT_ERR_HIP;
+        hipLaunchKernelGGL((k_mx_tn<FMT, T, SCALED, MT, NT, WM, WN, VEC, true>), grid, dim3(S::kThreads), S::kLds, st, a, td, tk);
         const int64_t total = (int64_t)a.Da * a.Db;
-        hipLaunchKernelGGL(k_mx_tn_join, dim3((unsigned)std::min<int64_t>((total + 255) / 256, 8 * vt_num_cu())), dim3(256), 0, st, a, p.slabs);
+        if (p.slabs <= 8)
+            hipLaunchKernelGGL(k_mx_tn_join_few, dim3((unsigned)std::min<int64_t>((total + 255) / 256, 8 * vt_num_cu())), dim3(256), 0, st, a, p.slabs);
+        else
+            hipLaunchKernelGGL(k_mx_tn_join<16>, dim3((unsigned)((total + 31) / 32)), dim3(512), 0, st, a, p.slabs);
     } else {
-        if (vt_allow_big_lds((const void*)k_mx_tn<FMT, T, SCALED, MT, NT, WM, WN, false>, attr_whole, S::kLds) != VT_OK) return VT_ERR_HIP;
-        hipLaunchKernelGGL((k_mx_tn<FMT, T, SCALED, MT, NT, WM, WN, false>), grid, dim3(S::kThreads), S::kLds, st, a);
+        if (vt_allow_big_lds((const void*)k_mx_tn<FMT, T, SCALED, MT, NT, WM, WN, VEC, false>, attr_whole, S::kLds) != VT_OK) return VT_ERR_HIP;
+        hipLaunchKernelGGL((k_mx_tn<FMT, T, SCALED, MT, NT, WM, WN, VEC, false>), grid, dim3(S::kThreads), S::kLds, st, a, td, tk);
     }
     return vt_launch_status();
 }
 
 template <int FMT, typename T, bool SCALED>
 int launch(const MxTN& a, const TnPlan& p, hipStream_t st) {
-    return p.bm == 256 ? launch<FMT, T, SCALED, 4, 2, 2, 2>(a, p, st) : launch<FMT, T, SCALED, 2, 1, 2, 2>(a, p, st);
+    const bool vec = (uintptr_t)a.B % 16 == 0 && a.ldb * (int64_t)sizeof(T) % 16 == 0;
+    if (p.bn == 256) return vec ? launch<FMT, T, SCALED, 4, 2, 2, 4, true>(a, p, st) : launch<FMT, T, SCALED, 4, 2, 2, 4, false>(a, p, st);
+    if (p.bm == 256) return vec ? launch<FMT, T, SCALED, 4, 2, 2, 2, true>(a, p, st) : launch<FMT, T, SCALED, 4, 2, 2, 2, false>(a, p, st);
+    return vec ? launch<FMT, T, SCALED, 2, 1, 2, 2, true>(a, p, st) : launch<FMT, T, SCALED, 2, 1, 2, 2, false>(a, p, st);
 }
 
 template <int FMT, typename T>
@@ -297,9 +370,9 @@ extern "C" int vt_mx_gemm_tn(int format, const void* codes, int64_t ldc, const v
     if (type < VT_TYPE_F32 || type > VT_TYPE_F16 || (N > 0 && (!B || ldb < Db))) return VT_ERR_BAD_ARG;
     const TnPlan p = plan(N, Da, Db);
     if (!ws || ws_bytes < vt_mx_gemm_tn_workspace_bytes(N, Da, Db)) return VT_ERR_WORKSPACE;
-    if ((Db + p.bn - 1) / p.bn > 65535) return VT_ERR_UNSUPPORTED;
-    const int64_t es = type == VT_TYPE_F32 ? 4 : 2;
-    const bool vec = (uintptr_t)B % 16 == 0 && ldb * es % 16 == 0;
-    MxTN a{(const uint8_t*)codes, (const uint8_t*)scales, ldc, lds, N, p.rows, Da, Db, B, ldb, vec, rowscale, alpha, bias, C, ldo, (float*)ws};
+    // 32-bit offsets inside a chunk of 32 rows, tile numbers in 31 bits
+    if (ldc >= 1 << 25 || lds >= 1 << 25 || (N > 1 && ldb >= 1 << 23)) return VT_ERR_UNSUPPORTED;
+    if ((int64_t)((Da + p.bm - 1) / p.bm) * ((Db + p.bn - 1) / p.bn) * p.slabs > 0x7ffffff0) return VT_ERR_UNSUPPORTED;
+    MxTN a{(const uint8_t*)codes, (const uint8_t*)scales, ldc, lds, N, p.rows, Da, Db, B, ldb, rowscale, alpha, bias, C, ldo, (float*)ws};
     return format == VT_MX_FP8 ? launch<VT_MX_FP8>(type, a, p, (hipStream_t)stream) : launch<VT_MX_FP4>(type, a, p, (hipStream_t)stream);
 }
