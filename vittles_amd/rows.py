@@ -2,7 +2,7 @@
 import torch
 
 from . import _lib, device as dev
-from .compact import CompactRows, TYPE as _MX_TYPE, on_device
+from .compact import CompactRows, TYPE as _MX_TYPE, on_device, stream_of
 
 _ws_cache = {}
 
@@ -57,14 +57,14 @@ def _vector(t, n, X, what):
 
 
 def _compact(name, X, lead, tail):
-    """``vt_mx_<name>`` on compact rows: (lead, format, codes, ldc, scales, lds, tail, workspace, stream).  The workspace
+    """The entry point ``name`` on compact rows: (lead, format, codes, ldc, scales, lds, tail, workspace, stream).  The workspace
     belongs to the call (and, under capture, to the graph): two graphs never share one."""
     lib = dev.require_gpu()
-    with on_device(X.device):
+    device = X.device
+    with on_device(device):
         nbytes = lib.vt_mx_rows_workspace_bytes(*X.shape)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=X.device)
-        _lib.check(getattr(lib, "vt_mx_" + name)(*lead, X.c_format(), *X.c_args(), *tail, ws.data_ptr(), nbytes,
-                                                 dev.stream_ptr()), "vt_mx_" + name)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        _lib.check(getattr(lib, name)(*lead, X.c_format(), *X.c_args(), *tail, ws.data_ptr(), nbytes, stream_of(device)), name)
 
 
 def _compact_glm(name, obj, theta, w, outs, prior=()):
@@ -110,7 +110,7 @@ def gemv(A, v):
     if isinstance(A, CompactRows):
         v = _vector(v, A.D, A, "v")
         out = torch.empty(A.shape[0], dtype=torch.float64, device=A.device)
-        _compact("gemv", A, (), (v.data_ptr(), *A.shape, out.data_ptr()))
+        _compact("vt_mx_gemv", A, (), (v.data_ptr(), *A.shape, out.data_ptr()))
         return out
     lib = dev.require_gpu()
     A = _rowmajor(A)
@@ -129,7 +129,7 @@ def gemv_t2(A, u1, u2):
         u1 = _vector(u1, A.shape[0], A, "u1")
         u2 = None if u2 is None else _vector(u2, A.shape[0], A, "u2")
         out = torch.empty(A.D, dtype=torch.float64, device=A.device)
-        _compact("gemv_t", A, (), (u1.data_ptr(), dev.ptr(u2), *A.shape, out.data_ptr()))
+        _compact("vt_mx_gemv_t", A, (), (u1.data_ptr(), dev.ptr(u2), *A.shape, out.data_ptr()))
         return out
     lib = dev.require_gpu()
     A = _rowmajor(A)
@@ -277,7 +277,7 @@ def _compact_gemm_tn(A, B, rowscale, alpha, bias, out):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=A.device)
         _lib.check(lib.vt_mx_gemm_tn(A.c_format(), *A.c_args(), Da, _MX_TYPE[B.dtype], B.data_ptr(), dev.ld(B), Db,
                                      dev.ptr(rowscale), N, float(alpha), dev.ptr(bias), out.data_ptr(), dev.ld(out),
-                                     ws.data_ptr(), nbytes, dev.stream_ptr()), "vt_mx_gemm_tn")
+                                     ws.data_ptr(), nbytes, stream_of(A.device)), "vt_mx_gemm_tn")
     return out
 
 
@@ -294,10 +294,10 @@ def gemm_nt(A, B, alpha=1.0, bias=None, out=None):
     out = _matrix_out(out, (M, N), (torch.float32, torch.bfloat16), A.device)
     with on_device(A.device):
         nbytes = lib.vt_mx_gemm_nt_workspace_bytes(M, N, A.D)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=A.device)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=A.device) if nbytes else None
         _lib.check(lib.vt_mx_gemm_nt(*A.c_args(), M, *B.c_args(), N, A.D, float(alpha), dev.ptr(bias),
-                                     _MX_TYPE[out.dtype], out.data_ptr(), dev.ld(out), ws.data_ptr(), nbytes,
-                                     dev.stream_ptr()), "vt_mx_gemm_nt")
+                                     _MX_TYPE[out.dtype], out.data_ptr(), dev.ld(out), dev.ptr(ws), nbytes,
+                                     stream_of(A.device)), "vt_mx_gemm_nt")
     return out
 
 
@@ -326,7 +326,7 @@ def glm_link(obj, theta, w, want_z=False):
     r = torch.empty(obj.N, dtype=torch.float64, device=obj.device)
     d = torch.empty(obj.N, dtype=torch.float64, device=obj.device)
     if isinstance(obj.X, CompactRows):
-        _compact_glm("glm_link", obj, theta, w, (z, r, d))
+        _compact_glm("vt_mx_glm_link", obj, theta, w, (z, r, d))
         return z, r, d
     ws = _workspace(obj.D, obj.device)
     _lib.check(_lib.fn(lib, "vt_glm_link", obj.X)(_lib.FAMILY[obj.family], obj.X.data_ptr(), dev.ld(obj.X), theta.data_ptr(),
@@ -346,7 +346,7 @@ def glm_grad(obj, theta, w, prior=None):
     d = torch.empty(obj.N, dtype=torch.float64, device=obj.device)
     if isinstance(obj.X, CompactRows):
         prior = None if prior is None else _vector(prior, obj.D, obj.X, "prior")
-        _compact_glm("glm_grad", obj, theta, w, (g, r, d), prior=(prior,))
+        _compact_glm("vt_mx_glm_grad", obj, theta, w, (g, r, d), prior=(prior,))
         return g, r, d
     ws = _workspace(obj.D, obj.device)
     _lib.check(_lib.fn(lib, "vt_glm_grad", obj.X)(_lib.FAMILY[obj.family], obj.X.data_ptr(), dev.ld(obj.X), theta.data_ptr(),
@@ -366,7 +366,7 @@ def glm_hvp(X, d, v, prior=None, prior_scalar=0.0, out=None):
             out = torch.empty(D, dtype=torch.float64, device=X.device)
         elif out.dtype != torch.float64 or out.shape != (D,) or out.device != X.device or not out.is_contiguous():
             raise ValueError("out must be a contiguous float64 tensor of shape (%d,) on %s" % (D, X.device))
-        _compact("glm_hvp", X, (), (d.data_ptr(), dev.ptr(prior), float(prior_scalar), v.data_ptr(), N, D, out.data_ptr()))
+        _compact("vt_mx_glm_hvp", X, (), (d.data_ptr(), dev.ptr(prior), float(prior_scalar), v.data_ptr(), N, D, out.data_ptr()))
         return out
     lib = dev.require_gpu()
     if out is None:
@@ -411,7 +411,7 @@ def glm_value(obj, theta, w):
     w = dev.to_device(w, obj.device).contiguous()
     val = torch.empty(1, dtype=torch.float64, device=obj.device)
     if isinstance(obj.X, CompactRows):
-        _compact_glm("glm_value", obj, theta, w, (val,))
+        _compact_glm("vt_mx_glm_value", obj, theta, w, (val,))
     else:
         ws = _workspace(obj.D, obj.device)
         _lib.check(_lib.fn(lib, "vt_glm_value", obj.X)(_lib.FAMILY[obj.family], obj.X.data_ptr(), dev.ld(obj.X), theta.data_ptr(),
