@@ -17,6 +17,12 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
+// 16 bytes at an element's own alignment (2, 4 or 8): the gfx950 ABI runs with unaligned wide accesses allowed.
+template <int ALIGN> struct Unaligned16;
+template <> struct Unaligned16<2> { typedef unsigned type __attribute__((ext_vector_type(4), aligned(2))); };
+template <> struct Unaligned16<4> { typedef unsigned type __attribute__((ext_vector_type(4), aligned(4))); };
+template <> struct Unaligned16<8> { typedef unsigned type __attribute__((ext_vector_type(4), aligned(8))); };
+
 __host__ __device__ __forceinline__ constexpr int mx_blocks(int D) { return D / kMxBlock + (D % kMxBlock != 0); }
 __host__ __device__ __forceinline__ constexpr int mx_block_bytes(int format) { return format == VT_MX_FP8 ? 32 : 16; }
 // codes in one 32-bit word
@@ -50,6 +56,15 @@ __device__ __forceinline__ void mx_word(unsigned word, float scale, float (&v)[k
         v[6] = p[0], v[7] = p[1];
     }
 }
+
+// A buffer descriptor of `bytes` from p on: loads past it give 0, stores past it are dropped.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_rsrc(const void* p, int64_t bytes) {
+    const uint64_t b = (uint64_t)p;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)b), hi = __builtin_amdgcn_readfirstlane((uint32_t)(b >> 32));
+    const uint32_t n = bytes <= 0 ? 0 : (uint32_t)std::min<int64_t>(bytes, 0x7fffffff);
+    return __builtin_amdgcn_make_buffer_rsrc((void*)(((uint64_t)hi << 32) | lo), 0, __builtin_amdgcn_readfirstlane(n), 0x00020000);
+}
+constexpr unsigned kNowhere = 0x80000000u;       // an offset past every descriptor
 
 // Host-side check of a compact matrix, shared by every entry point.
 inline bool mx_rows_ok(int format, const void* codes, int64_t ldc, const void* scales, int64_t lds, int64_t N, int D) {

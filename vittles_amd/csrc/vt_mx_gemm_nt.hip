@@ -4,6 +4,7 @@
 // they are stored.  E2M1 products times powers of two are exact and the sums are float (the E4M3 form of the instruction
 // keeps only about 17 bits of a sum: 8-bit rows are not multiplied this way).
 #include "vt_mx.h"
+#include <type_traits>
 
 namespace {
 
@@ -17,6 +18,7 @@ struct MxNT {
     const float* bias;
     void* C;
     int64_t ldc;
+    bool lines;                         // C's rows begin on cache lines
     float* part;                        // [slices][M][N] sums, when the axis is split
 };
 
@@ -27,8 +29,7 @@ __device__ __forceinline__ i32x8 nt_operand(u32x4 w) {
 
 template <typename OutT>
 __device__ __forceinline__ void mx_store(const MxNT& a, int64_t m, int64_t n, float v) {
-    // past the caches: C is not read again here (2048 x 4096 x 4096: 35.1 -> 32.5 us)
-    __builtin_nontemporal_store((OutT)(a.alpha * v + (a.bias ? a.bias[n] : 0.0f)), (OutT*)a.C + m * a.ldc + n);
+    ((OutT*)a.C)[m * a.ldc + n] = (OutT)(a.alpha * v + (a.bias ? a.bias[n] : 0.0f));
 }
 
 // ---- tiles ----------------------------------------------------------------------------------------------------------
@@ -47,25 +48,20 @@ __device__ __forceinline__ int nt_slot(int block, int row) { return 16 * (block 
 
 typedef __attribute__((address_space(3))) void* mx_ldsptr;
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_rsrc(const void* p, unsigned bytes) {
-    const uint64_t b = (uint64_t)p;
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)b), hi = __builtin_amdgcn_readfirstlane((uint32_t)(b >> 32));
-    return __builtin_amdgcn_make_buffer_rsrc((void*)(((uint64_t)hi << 32) | lo), 0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
-}
-
 template <int MT, int NT, int WM, int WN>
 struct NtShape {
     static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves, BM = 32 * MT * WM, BN = 32 * NT * WN;
     static constexpr int kCodes = (BM + BN) * 16 * kChunk, kBuf = kCodes + (BM + BN) * kChunk, kLds = 2 * kBuf;
     static constexpr int kLoadsA = BM / (kRowsPerLoad * kWaves), kLoadsB = BN / (kRowsPerLoad * kWaves),
-                         kLoadsS = (BM + BN) * (kChunk / 4) / (64 * kWaves);
-    static constexpr int kLoads = kLoadsA + kLoadsB + kLoadsS;      // of a wave for one chunk
-    static_assert(BM % (kRowsPerLoad * kWaves) == 0 && BN % (kRowsPerLoad * kWaves) == 0 && (BM + BN) * (kChunk / 4) % (64 * kWaves) == 0 && BM % 64 == 0, "even shares");
+                         kLoadsS = (BM + BN) * (kChunk / 4) / kThreads;      // of a wave for one chunk
+    static_assert(BM % (kRowsPerLoad * kWaves) == 0 && BN % (kRowsPerLoad * kWaves) == 0 && BM + BN == kThreads, "even shares, one row of scales a thread");
 };
 
-template <int MT, int NT, int WM, int WN, typename OutT, bool SPLIT>
+// DMA: the scales' rows all begin on 4 bytes and their words come by DMA too; else through registers (10 % slower).
+template <int MT, int NT, int WM, int WN, bool DMA, typename OutT, bool SPLIT>
 __global__ __launch_bounds__(64 * WM * WN) void k_mx_nt_tile(MxNT a, int tiles_m, int tiles_n) {
     using S = NtShape<MT, NT, WM, WN>;
+    constexpr int kLoadsA = S::kLoadsA, kLoadsB = S::kLoadsB, kLoads = kLoadsA + kLoadsB + (DMA ? S::kLoadsS : 0), kWords = kChunk / 4, kScaleRows = 64 / kWords;
     extern __shared__ __align__(16) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WN, wn = wave % WN;
@@ -81,30 +77,40 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_nt_tile(MxNT a, int tiles_m
 
     const int rows_a = (int)std::min<int64_t>(S::BM, a.M - m0), rows_b = (int)std::min<int64_t>(S::BN, a.N - n0);
     // rows past the end read 0; blocks past a row's end are the next row's, and are masked in the last chunk
-    const auto ra = mx_rsrc(a.ca + m0 * a.ldca, (unsigned)((rows_a - 1) * a.ldca + 16 * (int64_t)a.nb));
-    const auto rb = mx_rsrc(a.cb + n0 * a.ldcb, (unsigned)((rows_b - 1) * a.ldcb + 16 * (int64_t)a.nb));
-    // (a scale word that holds a row's last scale may reach up to three bytes behind it, never out of its own 4 bytes)
-    const auto rsa = mx_rsrc(a.sa + m0 * a.ldsa, (unsigned)((rows_a - 1) * a.ldsa + (a.nb + 3) / 4 * 4));
-    const auto rsb = mx_rsrc(a.sb + n0 * a.ldsb, (unsigned)((rows_b - 1) * a.ldsb + (a.nb + 3) / 4 * 4));
+    const auto ra = mx_rsrc(a.ca + m0 * a.ldca, (rows_a - 1) * a.ldca + 16 * (int64_t)a.nb);
+    const auto rb = mx_rsrc(a.cb + n0 * a.ldcb, (rows_b - 1) * a.ldcb + 16 * (int64_t)a.nb);
     const int rl = lane / kChunk, piece = nt_slot(lane % kChunk, rl + kRowsPerLoad * wave);     // (kWaves is even)
     const unsigned va = rl * (unsigned)a.ldca + piece, vb = rl * (unsigned)a.ldcb + piece;
-    constexpr int kWords = kChunk / 4, kScaleRows = 64 / kWords;
+    // (a scale word that holds a row's last scale may reach up to three bytes behind it, never out of its own 4 bytes)
+    const auto rsa = mx_rsrc(a.sa + m0 * a.ldsa, (rows_a - 1) * a.ldsa + (a.nb + 3) / 4 * 4);
+    const auto rsb = mx_rsrc(a.sb + n0 * a.ldsb, (rows_b - 1) * a.ldsb + (a.nb + 3) / 4 * 4);
     const unsigned vsa = lane / kWords * (unsigned)a.ldsa + 4 * (lane % kWords), vsb = lane / kWords * (unsigned)a.ldsb + 4 * (lane % kWords);
+    // not DMA: this thread's row of scales; rows past the end repeat the last one
+    const uint8_t* const ps = tid < S::BM ? a.sa + (m0 + std::min(tid, rows_a - 1)) * a.ldsa : a.sb + (n0 + std::min(tid - S::BM, rows_b - 1)) * a.ldsb;
 
     // load number i of this wave for the chunk at block kb
     auto fetch = [&](int kb, uint8_t* base, int i) {
-        if (i < S::kLoadsA) {
+        if (i < kLoadsA) {
             const int row = kRowsPerLoad * (wave + S::kWaves * i);
             __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (mx_ldsptr)(base + row * kRow), 16, va + row * (unsigned)a.ldca + 16u * kb, 0, 0, 0);
-        } else if (i < S::kLoadsA + S::kLoadsB) {
-            const int row = kRowsPerLoad * (wave + S::kWaves * (i - S::kLoadsA));
+        } else if (i < kLoadsA + kLoadsB) {
+            const int row = kRowsPerLoad * (wave + S::kWaves * (i - kLoadsA));
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (mx_ldsptr)(base + (S::BM + row) * kRow), 16, vb + row * (unsigned)a.ldcb + 16u * kb, 0, 0, 0);
         } else {
-            const int row = kScaleRows * (wave + S::kWaves * (i - S::kLoadsA - S::kLoadsB));
+            const int row = kScaleRows * (wave + S::kWaves * (i - kLoadsA - kLoadsB));
             const bool first = row < S::BM;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(first ? rsa : rsb, (mx_ldsptr)(base + S::kCodes + row * kChunk), 4,
                                                      (first ? vsa + row * (unsigned)a.ldsa : vsb + (row - S::BM) * (unsigned)a.ldsb) + kb, 0, 0, 0);
         }
+    };
+    // the eight scale bytes of its chunk, at whatever address they lie; blocks past the row's end count as 1
+    auto scales = [&](int kb) -> u32x2 {
+        typedef unsigned u32x2u __attribute__((ext_vector_type(2), aligned(1)));
+        if (kb + kChunk <= a.nb) return *(const u32x2u*)(ps + kb);
+        uint64_t v = 0;
+#pragma unroll 1
+        for (int j = 0; j < kChunk; ++j) v |= (uint64_t)(kb + j < a.nb ? ps[kb + j] : 127) << (8 * j);
+        return __builtin_bit_cast(u32x2, v);
     };
 
     f32x16 acc[MT][NT];
@@ -141,8 +147,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_nt_tile(MxNT a, int tiles_m
             for (int j = 0; j < NT; ++j) fb[j] = nt_operand(*(const u32x4*)(pb + 32 * kRow * j + slot));
             if (more) {
 #pragma unroll
-                for (int i = 0; i < S::kLoads; ++i)
-                    if (i * 2 / S::kLoads == s) fetch(kb, next, i);
+                for (int i = 0; i < kLoads; ++i)
+                    if (i * 2 / kLoads == s) fetch(kb, next, i);
             }
 #pragma unroll
             for (int i = 0; i < MT; ++i)
@@ -158,8 +164,10 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_nt_tile(MxNT a, int tiles_m
         asm volatile("" ::: "memory");
     };
 
+    uint8_t* const scale_slot = lds + S::kCodes + tid * kChunk;
+    if constexpr (!DMA) *(u32x2*)scale_slot = scales(kb_lo);
 #pragma unroll
-    for (int i = 0; i < S::kLoads; ++i) fetch(kb_lo, lds, i);
+    for (int i = 0; i < kLoads; ++i) fetch(kb_lo, lds, i);
     for (int c = 0; c < chunks; ++c) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // this wave's part of chunk c has landed
         barrier();          // everybody's has, and chunk c - 1 has been read: its place is free
@@ -168,34 +176,51 @@ __global__ __launch_bounds__(64 * WM * WN) void k_mx_nt_tile(MxNT a, int tiles_m
         if (kb + kChunk > a.nb) {
             // the row ends inside this chunk: codes of A behind the end become 0 and scales 1, so that what was
             // fetched there (the next row's) counts for nothing
-            for (int i = tid; i < (S::BM + S::BN) * kChunk; i += S::kThreads) {
+            if constexpr (DMA)
+                for (int i = tid; i < (S::BM + S::BN) * kChunk; i += S::kThreads)
+                    if (kb + i % kChunk >= a.nb) base[S::kCodes + i] = 127;
+            for (int i = tid; i < S::BM * kChunk; i += S::kThreads) {
                 const int row = i / kChunk, j = i % kChunk;
-                if (kb + j < a.nb) continue;
-                base[S::kCodes + row * kChunk + j] = 127;
-                if (row < S::BM) *(u32x4*)(base + row * kRow + nt_slot(j, row)) = u32x4{0, 0, 0, 0};
+                if (kb + j >= a.nb) *(u32x4*)(base + row * kRow + nt_slot(j, row)) = u32x4{0, 0, 0, 0};
             }
             barrier();
         }
+        u32x2 next = {0, 0};
+        if constexpr (!DMA)
+            if (c + 1 < chunks) next = scales(kb + kChunk);
         multiply(base, c + 1 < chunks, kb + kChunk, lds + (~c & 1) * S::kBuf);
+        if (!DMA && c + 1 < chunks) *(u32x2*)(scale_slot + (~c & 1) * S::kBuf) = next;
     }
 
-    // lane, element e of a 32 x 32 result: row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32
+    // lane, element e of a 32 x 32 result: row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32; rows and columns past
+    // the end fall outside the descriptor
+    using T = typename std::conditional<SPLIT, float, OutT>::type;
+    const int64_t ld = SPLIT ? a.N : a.ldc;
+    T* const out = SPLIT ? (T*)(a.part + (int64_t)blockIdx.y * a.M * a.N) : (T*)a.C;
+    auto write = [&](auto aux) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+        for (int i = 0; i < MT; ++i) {
+            const int64_t m = m0 + 32 * (wm * MT + i);
+            const auto rc = mx_rsrc(out + m * ld + n0, m < a.M ? ((a.M - 1 - m) * ld + a.N - n0) * (int64_t)sizeof(T) : 0);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const int64_t n = n0 + 32 * (wn * NT + j) + l;
-            if (n < a.N) {
+            for (int j = 0; j < NT; ++j) {
+                const int n = 32 * (wn * NT + j) + l;
+                const float bias = !SPLIT && a.bias && n < rows_b ? a.bias[n0 + n] : 0.0f;
+                const unsigned at = n < rows_b ? (unsigned)sizeof(T) * (4 * h * (unsigned)ld + n) : kNowhere;
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    const int64_t m = m0 + 32 * (wm * MT + i) + 8 * (e / 4) + 4 * h + e % 4;
-                    if (m < a.M) {
-                        if constexpr (SPLIT) a.part[((int64_t)blockIdx.y * a.M + m) * a.N + n] = acc[i][j][e];
-                        else mx_store<OutT>(a, m, n, acc[i][j][e]);
-                    }
+                    const T c = (T)(SPLIT ? acc[i][j][e] : a.alpha * acc[i][j][e] + bias);
+                    const unsigned off = at + (unsigned)sizeof(T) * (8 * (e / 4) + e % 4) * (unsigned)ld;
+                    if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, c), rc, off, 0, decltype(aux)::value);
+                    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, c), rc, off, 0, decltype(aux)::value);
                 }
             }
         }
+    };
+    // whole lines go past the caches, C is not read again here (2048 x 4096 x 4096: 35.1 -> 32.5 us); parts of lines have
+    // to meet in L2 first (8192 x 8191 x 512: 202 us past it, 93 through it)
+    if (!SPLIT && a.lines) write(std::integral_constant<int, 2>());
+    else write(std::integral_constant<int, 0>());
 }
 
 template <typename OutT>
@@ -210,9 +235,10 @@ __global__ __launch_bounds__(256) void k_mx_nt_join(MxNT a, int slices) {
 }
 
 // ---- few rows -------------------------------------------------------------------------------------------------------
-// At most 16 MT rows on one side ("few", F): each wave streams 16 rows of the other side ("many") straight from memory
-// into v_mfma_scale_f32_16x16x128, four waves of a workgroup on interleaved chunks of the axis, joined through LDS.
-// Reading the many rows once is the whole cost.  SWAP: the few rows are B's.
+// Blocks of at most 16 MT rows of the shorter side ("few", F): each workgroup streams 16 rows of the other side ("many")
+// straight from memory into v_mfma_scale_f32_16x16x128, its four waves on interleaved chunks of the axis, joined through
+// LDS.  For up to 64 rows reading the many rows once is the whole cost; for small products with more it saves the tiles'
+// long way in and out (151 x 219 x 563: 13.5 us in tiles).  SWAP: the few rows are B's.
 struct MxFew {
     const uint8_t *cm, *sm, *cf, *sf;      // many, few
     int64_t ldcm, ldsm, ldcf, ldsf, many, few;
@@ -225,13 +251,13 @@ __global__ __launch_bounds__(256) void k_mx_nt_few(MxNT a, MxFew f) {
     constexpr int U = 4;                   // steps of 4 blocks a wave takes at once: 256 bytes a row
     __shared__ f32x4 sh[3][MT][64];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, q = lane >> 4;
-    const int64_t r0 = (int64_t)blockIdx.x * 16;
+    const int64_t r0 = (int64_t)blockIdx.x * 16, f0 = (int64_t)blockIdx.y * 16 * MT;
     const int64_t rm = std::min(r0 + l, f.many - 1);
     const uint8_t *pm = f.cm + rm * f.ldcm, *ps = f.sm + rm * f.ldsm;
     const uint8_t *pf[MT], *pfs[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-        const int64_t r = std::min<int64_t>(16 * i + l, f.few - 1);
+        const int64_t r = std::min<int64_t>(f0 + 16 * i + l, f.few - 1);
         pf[i] = f.cf + r * f.ldcf;
         pfs[i] = f.sf + r * f.ldsf;
     }
@@ -274,7 +300,7 @@ __global__ __launch_bounds__(256) void k_mx_nt_few(MxNT a, MxFew f) {
         // element e: many row 4 q + e, few row l
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int64_t m = r0 + 4 * q + e, k = 16 * i + l;
+            const int64_t m = r0 + 4 * q + e, k = f0 + 16 * i + l;
             if (m < f.many && k < f.few) mx_store<OutT>(a, SWAP ? m : k, SWAP ? k : m, v[e]);
         }
     }
@@ -285,23 +311,10 @@ int launch_few(const MxNT& a, hipStream_t st) {
     const bool swap = a.N < a.M;
     MxFew f = swap ? MxFew{a.ca, a.sa, a.cb, a.sb, a.ldca, a.ldsa, a.ldcb, a.ldsb, a.M, a.N}
                    : MxFew{a.cb, a.sb, a.ca, a.sa, a.ldcb, a.ldsb, a.ldca, a.ldsa, a.N, a.M};
-    const dim3 grid((unsigned)((f.many + 15) / 16));
+    const dim3 grid((unsigned)((f.many + 15) / 16), (unsigned)((f.few + 16 * MT - 1) / (16 * MT)));
     if (swap) hipLaunchKernelGGL((k_mx_nt_few<MT, true, OutT>), grid, dim3(256), 0, st, a, f);
     else hipLaunchKernelGGL((k_mx_nt_few<MT, false, OutT>), grid, dim3(256), 0, st, a, f);
     return vt_launch_status();
-}
-
-// Scale rows that do not start on 4 bytes, copied to rows that do (the DMA takes a row's four scale bytes at once).
-__global__ __launch_bounds__(256) void k_mx_nt_scales(const uint8_t* s, int64_t lds, int64_t rows, int nb, unsigned* out) {
-    const int words = (nb + 3) / 4;
-    const int64_t total = rows * words;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / words;
-        const int w = (int)(i - r * words);
-        unsigned v = 0;
-        for (int j = 0; j < 4; ++j) v |= (unsigned)(4 * w + j < nb ? s[r * lds + 4 * w + j] : 127) << (8 * j);
-        out[i] = v;
-    }
 }
 
 struct NtPlan {
@@ -312,39 +325,36 @@ struct NtPlan {
 
 int64_t tiles(int64_t M, int64_t N, int bm, int bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); }
 
-NtPlan plan(int64_t M, int64_t N, int K) {
+NtPlan plan(int64_t M, int64_t N, int K, bool far) {
     const int nb = mx_blocks(K);
     NtPlan p{0, 1, 1, (nb + kChunk - 1) / kChunk * kChunk};
-    const int64_t less = std::min(M, N);
-    if (less <= 64) {
-        p.few = (int)((less + 15) / 16);
+    const int64_t less = std::min(M, N), more = std::max(M, N);
+    // a few rows' workgroup reads its few rows again for every 16 of the many: up to 48 MB of that from L2 it is the faster
+    const double again = 0.5 * K * ((double)((more + 15) / 16) * less + (double)((less + 63) / 64) * more);
+    if (less <= 64 || again <= 48e6 || far) {
+        p.few = less <= 64 ? (int)((less + 15) / 16) : 4;
         return p;
     }
+    // Tiles: 256 x 256, one to a CU, or 128 x 128, two.  A round of them took about 18 + 2 us a chunk in the first (4096^2 and
+    // 8192^2, 256 to 8192 columns), 12 + 1.3 in the second; it says 47 against 33 us at 2048 x 4096 x 4096 and 82 against
+    // 107 at 4096 x 4096 x 8192, measured 47, 33, 82 and 105.
     const int cu = vt_num_cu();
-    // 256 x 256 tiles read the fewest bytes a product (8192^3: 320 against 389 us in 128 x 128), but a workgroup fills a
-    // CU: with fewer tiles than CUs the smaller ones, two to a CU, are faster (2048 x 4096 x 4096: 33 against 47 us)
-    p.shape = tiles(M, N, 256, 256) >= cu ? 0 : 1;
+    const int chunks = (nb + kChunk - 1) / kChunk;
+    const int64_t t = tiles(M, N, 128, 128);
+    const double big = (double)((tiles(M, N, 256, 256) + cu - 1) / cu) * (18.0 + 2.0 * chunks);
+    const double small = (double)((t + 2 * cu - 1) / (2 * cu)) * (12.0 + 1.3 * chunks);
+    p.shape = big < small ? 0 : 1;
     // few tiles and a long axis: slices of at least 8 chunks, joined by a second pass (300 x 300 x 8192: 32 us whole, 20
     // in four slices; 512 x 4096 x 4096, 128 tiles: 23 us whole, 27 in two)
-    const int64_t t = tiles(M, N, 128, 128);
-    const int chunks = (nb + kChunk - 1) / kChunk;
-    const int s = p.shape == 0 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(cu / (2 * t), chunks / 8));
+    const int s = p.shape == 0 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(cu / (2 * t), chunks / 8), 16));
     p.step = (chunks + s - 1) / s * kChunk;
     p.slices = (nb + p.step - 1) / p.step;
     return p;
 }
 
-bool scales_ready(const void* s, int64_t ld) { return (uintptr_t)s % 4 == 0 && ld % 4 == 0 && ld < 1 << 23; }
-size_t padded_scales(int64_t rows, int nb) { return ((size_t)rows * ((nb + 3) / 4) * 4 + 255) / 256 * 256; }
+bool scale_words(const void* s, int64_t ld) { return (uintptr_t)s % 4 == 0 && ld % 4 == 0 && ld < 1 << 23; }
 
-const uint8_t* repack(const uint8_t* s, int64_t ld, int64_t rows, int nb, uint8_t* to, hipStream_t st) {
-    const int64_t words = rows * ((nb + 3) / 4);
-    hipLaunchKernelGGL(k_mx_nt_scales, dim3((unsigned)std::min<int64_t>((words + 255) / 256, 8 * vt_num_cu())), dim3(256), 0, st, s, ld,
-                       rows, nb, (unsigned*)to);
-    return to;
-}
-
-template <int MT, int NT, int WM, int WN, typename OutT>
+template <int MT, int NT, int WM, int WN, bool DMA, typename OutT>
 int launch_tile(const MxNT& a, const NtPlan& p, hipStream_t st) {
     using S = NtShape<MT, NT, WM, WN>;
     const int tm = (int)((a.M + S::BM - 1) / S::BM), tn = (int)((a.N + S::BN - 1) / S::BN);
@@ -352,13 +362,13 @@ int launch_tile(const MxNT& a, const NtPlan& p, hipStream_t st) {
     const dim3 grid((unsigned)wgs, p.slices);
     static VtLdsAttr attr_split, attr_whole;
     if (p.slices > 1) {
-        if (vt_allow_big_lds((const void*)k_mx_nt_tile<MT, NT, WM, WN, OutT, true>, attr_split, S::kLds) != VT_OK) return VT_ERR_HIP;
-        hipLaunchKernelGGL((k_mx_nt_tile<MT, NT, WM, WN, OutT, true>), grid, dim3(S::kThreads), S::kLds, st, a, tm, tn);
+        if (vt_allow_big_lds((const void*)k_mx_nt_tile<MT, NT, WM, WN, DMA, OutT, true>, attr_split, S::kLds) != VT_OK) return VT_ERR_HIP;
+        hipLaunchKernelGGL((k_mx_nt_tile<MT, NT, WM, WN, DMA, OutT, true>), grid, dim3(S::kThreads), S::kLds, st, a, tm, tn);
         hipLaunchKernelGGL((k_mx_nt_join<OutT>), dim3((unsigned)std::min<int64_t>((a.M * a.N + 255) / 256, 8 * vt_num_cu())),
                            dim3(256), 0, st, a, p.slices);
     } else {
-        if (vt_allow_big_lds((const void*)k_mx_nt_tile<MT, NT, WM, WN, OutT, false>, attr_whole, S::kLds) != VT_OK) return VT_ERR_HIP;
-        hipLaunchKernelGGL((k_mx_nt_tile<MT, NT, WM, WN, OutT, false>), grid, dim3(S::kThreads), S::kLds, st, a, tm, tn);
+        if (vt_allow_big_lds((const void*)k_mx_nt_tile<MT, NT, WM, WN, DMA, OutT, false>, attr_whole, S::kLds) != VT_OK) return VT_ERR_HIP;
+        hipLaunchKernelGGL((k_mx_nt_tile<MT, NT, WM, WN, DMA, OutT, false>), grid, dim3(S::kThreads), S::kLds, st, a, tm, tn);
     }
     return vt_launch_status();
 }
@@ -372,19 +382,17 @@ int launch(const MxNT& a, const NtPlan& p, hipStream_t st) {
         case 3: return launch_few<3, OutT>(a, st);
         default: return launch_few<4, OutT>(a, st);
     }
-    switch (p.shape) {
-        case 0: return launch_tile<4, 2, 2, 4, OutT>(a, p, st);
-        default: return launch_tile<2, 2, 2, 2, OutT>(a, p, st);
-    }
+    const bool dma = scale_words(a.sa, a.ldsa) && scale_words(a.sb, a.ldsb);
+    if (p.shape == 0) return dma ? launch_tile<4, 2, 2, 4, true, OutT>(a, p, st) : launch_tile<4, 2, 2, 4, false, OutT>(a, p, st);
+    return dma ? launch_tile<2, 2, 2, 2, true, OutT>(a, p, st) : launch_tile<2, 2, 2, 2, false, OutT>(a, p, st);
 }
 
 }  // namespace
 
 extern "C" size_t vt_mx_gemm_nt_workspace_bytes(int64_t M, int64_t N, int K) {
     if (M < 1 || N < 1 || K < 1) return 0;
-    const NtPlan p = plan(M, N, K);
-    if (p.few > 0) return 0;
-    return padded_scales(M, mx_blocks(K)) + padded_scales(N, mx_blocks(K)) + (p.slices > 1 ? (size_t)p.slices * M * N * sizeof(float) : 0);
+    const NtPlan p = plan(M, N, K, false);
+    return p.few == 0 && p.slices > 1 ? (size_t)p.slices * M * N * sizeof(float) : 0;
 }
 
 extern "C" int vt_mx_gemm_nt(const void* ca, int64_t ldca, const void* sa, int64_t ldsa, int64_t M, const void* cb,
@@ -395,17 +403,11 @@ extern "C" int vt_mx_gemm_nt(const void* ca, int64_t ldca, const void* sa, int64
     if (out_type != VT_TYPE_F32 && out_type != VT_TYPE_BF16) return VT_ERR_BAD_ARG;
     if (M == 0 || N == 0) return VT_OK;
     if (!C || ldc < N) return VT_ERR_BAD_ARG;
-    // 32-bit offsets inside a tile of 256 rows, tile numbers in 31 bits
-    if (ldca >= 1 << 23 || ldcb >= 1 << 23 || tiles(M, N, 128, 16) > 0x7ffffff0) return VT_ERR_UNSUPPORTED;
+    if (tiles(M, N, 16, 64) > 0x7ffffff0) return VT_ERR_UNSUPPORTED;
     if (ws_bytes < vt_mx_gemm_nt_workspace_bytes(M, N, K) || (!ws && vt_mx_gemm_nt_workspace_bytes(M, N, K))) return VT_ERR_WORKSPACE;
-    const NtPlan p = plan(M, N, K);
+    // (a tile's offsets are 32 bits: 256 rows of codes, 32 rows of C)
+    const NtPlan p = plan(M, N, K, ldca >= 1 << 23 || ldcb >= 1 << 23 || ldc >= 1 << 24);
     MxNT a{(const uint8_t*)ca, (const uint8_t*)sa, (const uint8_t*)cb, (const uint8_t*)sb, ldca, ldsa, ldcb, ldsb, M, N,
-           mx_blocks(K), p.step, alpha, bias, C, ldc, nullptr};
-    if (p.few == 0) {
-        const size_t wa = padded_scales(M, a.nb), wb = padded_scales(N, a.nb);
-        if (!scales_ready(sa, ldsa)) a.sa = repack(a.sa, a.ldsa, M, a.nb, (uint8_t*)ws, (hipStream_t)stream), a.ldsa = (a.nb + 3) / 4 * 4;
-        if (!scales_ready(sb, ldsb)) a.sb = repack(a.sb, a.ldsb, N, a.nb, (uint8_t*)ws + wa, (hipStream_t)stream), a.ldsb = (a.nb + 3) / 4 * 4;
-        a.part = (float*)((uint8_t*)ws + wa + wb);
-    }
+           mx_blocks(K), p.step, alpha, bias, C, ldc, (uintptr_t)C % 128 == 0 && ldc * (out_type == VT_TYPE_F32 ? 4 : 2) % 128 == 0, (float*)ws};
     return out_type == VT_TYPE_F32 ? launch<float>(a, p, (hipStream_t)stream) : launch<__bf16>(a, p, (hipStream_t)stream);
 }

@@ -67,15 +67,6 @@ __device__ __forceinline__ s16x8 read_tr(const uint8_t* p, int next4) {
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// A descriptor that ends `bytes` behind p; loads past it give 0.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t tn_rsrc(const void* base, int64_t bytes) {
-    const uint64_t p = (uint64_t)base;
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)p), hi = __builtin_amdgcn_readfirstlane((uint32_t)(p >> 32));
-    const uint32_t n = bytes <= 0 ? 0 : (uint32_t)std::min<int64_t>(bytes, 0x7fffffff);
-    return __builtin_amdgcn_make_buffer_rsrc((void*)(((uint64_t)hi << 32) | lo), 0, __builtin_amdgcn_readfirstlane(n), 0x00020000);
-}
-constexpr unsigned kNowhere = 0x80000000u;       // an offset past every descriptor
-
 template <int FMT, typename T, bool SCALED, int MT, int NT, int WM, int WN, bool VEC, bool SPLIT>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tn(MxTN a, int tiles_d, int tiles_k) {
     constexpr int PARTS = kParts<T, SCALED>;
@@ -115,10 +106,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tn(MxTN a, int tiles_d, 
     // of the tile that are not stored
     auto fetch = [&](int64_t n0, Chunk& x) {
         const int64_t left = n_hi - n0;
-        const auto ra = tn_rsrc(a.codes + n0 * a.ldc, left > 0 ? (left - 1) * a.ldc + (FMT == VT_MX_FP8 ? width : width / 2) : 0);
-        const auto rs = tn_rsrc(a.scales + n0 * a.lds, left > 0 ? (left - 1) * a.lds + width / kMxBlock : 0);
+        const auto ra = mx_rsrc(a.codes + n0 * a.ldc, left > 0 ? (left - 1) * a.ldc + (FMT == VT_MX_FP8 ? width : width / 2) : 0);
+        const auto rs = mx_rsrc(a.scales + n0 * a.lds, left > 0 ? (left - 1) * a.lds + width / kMxBlock : 0);
         const int64_t last = VEC ? (a.Db + 7) / 8 * 8 : a.Db;
-        const auto rb = tn_rsrc((const T*)a.B + n0 * a.ldb, left > 0 ? ((left - 1) * a.ldb + last) * (int64_t)sizeof(T) : 0);
+        const auto rb = mx_rsrc((const T*)a.B + n0 * a.ldb, left > 0 ? ((left - 1) * a.ldb + last) * (int64_t)sizeof(T) : 0);
 #pragma unroll
         for (int i = 0; i < S::kLoadsA; ++i) {
             if constexpr (FMT == VT_MX_FP8) x.ca[i] = __builtin_bit_cast(W, __builtin_amdgcn_raw_buffer_load_b128(ra, va[i], 0, 0));
@@ -132,13 +123,22 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tn(MxTN a, int tiles_d, 
                 for (int j = 0; j < (int)sizeof(T) / 2; ++j)
                     x.cb[i][j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rb, vb[i] + 16 * j, 0, 0));
             } else {
-                T v[8];
+                // rows at any alignment: wide loads at the element's own, single ones at the row's end
+                typedef typename Unaligned16<sizeof(T)>::type wide;
+                const int e = tid + S::kThreads * i, c = k0 + e % (S::BN / 8) * 8;
+                const int64_t n = n0 + e / (S::BN / 8);
+                const T* p = (const T*)a.B + n * a.ldb + c;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    if constexpr (sizeof(T) == 4) v[j] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(rb, vb[i] + 4 * j, 0, 0));
-                    else v[j] = __builtin_bit_cast(T, (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(rb, vb[i] + 2 * j, 0, 0));
+                for (int j = 0; j < (int)sizeof(T) / 2; ++j) x.cb[i][j] = u32x4{0, 0, 0, 0};
+                if (n < n_hi && c + 8 <= a.Db) {
+#pragma unroll
+                    for (int j = 0; j < (int)sizeof(T) / 2; ++j) x.cb[i][j] = ((const wide*)p)[j];
+                } else if (n < n_hi && c < a.Db) {
+                    T v[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = c + j < a.Db ? p[j] : (T)0.0f;
+                    __builtin_memcpy(x.cb[i], v, sizeof(v));
                 }
-                __builtin_memcpy(x.cb[i], v, sizeof(v));
             }
             if constexpr (SCALED) {
                 const int64_t n = n0 + (tid + S::kThreads * i) / (S::BN / 8);
@@ -247,24 +247,27 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tn(MxTN a, int tiles_d, 
         put(even, lds);
     }
 
-    // lane, element e of a 32 x 32 result: row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32
+    // lane, element e of a 32 x 32 result: row 8 (e / 4) + 4 (lane / 32) + e % 4, column lane % 32; rows and columns past
+    // the end fall outside the descriptor
     const int l = lane & 31, h = lane >> 5;
+    const int64_t ld = SPLIT ? a.Db : a.ldo;
+    float* const out = SPLIT ? a.part + (int64_t)slab * a.Da * a.Db : a.C;
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < MT; ++i) {
+        const int d = d0 + 32 * (wm * MT + i);
+        const auto rc = mx_rsrc(out + d * ld + k0, d < a.Da ? ((a.Da - 1 - d) * ld + a.Db - k0) * (int64_t)sizeof(float) : 0);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            const int k = k0 + 32 * (wn * NT + j) + l;
-            if (k < a.Db) {
+            const int k = 32 * (wn * NT + j) + l;
+            const bool in = k0 + k < a.Db;
+            const float bias = !SPLIT && a.bias && in ? a.bias[k0 + k] : 0.0f;
+            const unsigned at = in ? 4 * (4 * h * (unsigned)ld + k) : kNowhere;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int d = d0 + 32 * (wm * MT + i) + 8 * (e / 4) + 4 * h + e % 4;
-                    if (d < a.Da) {
-                        if constexpr (SPLIT) a.part[((int64_t)slab * a.Da + d) * a.Db + k] = acc[i][j][e];
-                        else a.C[(int64_t)d * a.ldo + k] = a.alpha * acc[i][j][e] + (a.bias ? a.bias[k] : 0.0f);
-                    }
-                }
-            }
+            for (int e = 0; e < 16; ++e)
+                __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, SPLIT ? acc[i][j][e] : a.alpha * acc[i][j][e] + bias), rc,
+                                                      at + 4 * (8 * (e / 4) + e % 4) * (unsigned)ld, 0, 0);
         }
+    }
 }
 
 // The slabs' sums in a fixed order: 32 elements a workgroup, G groups of threads that each take every G-th slab.
@@ -306,9 +309,11 @@ struct TnPlan {
 
 TnPlan plan(int64_t N, int Da, int Db) {
     TnPlan p;
-    if (Db > 128) p.bm = 256, p.bn = 256;
-    else if (Db > 64) p.bm = 256, p.bn = 128;
-    else p.bm = 128, p.bn = 64;
+    // 128 x 64 tiles where a round or two of them with 128 rows each is the whole product: the way in and out of a tile of
+    // 256 x 256 alone takes longer
+    const int64_t small = (int64_t)((Da + 127) / 128) * ((Db + 63) / 64) * ((N + 127) / 128);
+    if (Db <= 64 || small <= 4 * vt_num_cu()) p.bm = 128, p.bn = 64;
+    else p.bm = 256, p.bn = Db > 128 ? 256 : 128;
     const int64_t tiles = (int64_t)((Da + p.bm - 1) / p.bm) * ((Db + p.bn - 1) / p.bn);
     const int64_t want = std::max<int64_t>(1, (p.bn == 256 ? 1 : 2) * vt_num_cu() / tiles), most = std::max<int64_t>(1, N / 128);
     p.slabs = (int)std::min(want, most);
@@ -370,8 +375,8 @@ extern "C" int vt_mx_gemm_tn(int format, const void* codes, int64_t ldc, const v
     if (type < VT_TYPE_F32 || type > VT_TYPE_F16 || (N > 0 && (!B || ldb < Db))) return VT_ERR_BAD_ARG;
     const TnPlan p = plan(N, Da, Db);
     if (!ws || ws_bytes < vt_mx_gemm_tn_workspace_bytes(N, Da, Db)) return VT_ERR_WORKSPACE;
-    // 32-bit offsets inside a chunk of 32 rows, tile numbers in 31 bits
-    if (ldc >= 1 << 25 || lds >= 1 << 25 || (N > 1 && ldb >= 1 << 23)) return VT_ERR_UNSUPPORTED;
+    // 32-bit offsets inside a chunk of 64 rows, tile numbers in 31 bits
+    if (ldc >= 1 << 25 || lds >= 1 << 25 || (N > 1 && ldb >= 1 << 23) || ldo >= 1 << 24) return VT_ERR_UNSUPPORTED;
     if ((int64_t)((Da + p.bm - 1) / p.bm) * ((Db + p.bn - 1) / p.bn) * p.slabs > 0x7ffffff0) return VT_ERR_UNSUPPORTED;
     MxTN a{(const uint8_t*)codes, (const uint8_t*)scales, ldc, lds, N, p.rows, Da, Db, B, ldb, rowscale, alpha, bias, C, ldo, (float*)ws};
     return format == VT_MX_FP8 ? launch<VT_MX_FP8>(type, a, p, (hipStream_t)stream) : launch<VT_MX_FP4>(type, a, p, (hipStream_t)stream);

@@ -18,13 +18,18 @@ typedef __bf16 bf16;
 constexpr int kPer = 8;
 
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, int valid, bool vec, T (&x)[kPer]) {
-    if (vec && valid == kPer) {
+struct Wide {
+    typedef typename Unaligned16<sizeof(T)>::type type;      // rows of odd length begin at any element
+};
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int valid, T (&x)[kPer]) {
+    if (valid == kPer) {
         constexpr int W = (int)sizeof(T) * kPer / 16;
-        u32x4 t[W];
+        typename Wide<T>::type t[W];
 #pragma unroll
-        for (int i = 0; i < W; ++i) t[i] = ((const u32x4*)p)[i];
-        __builtin_memcpy(x, t, sizeof(t));
+        for (int i = 0; i < W; ++i) t[i] = ((const typename Wide<T>::type*)p)[i];
+        __builtin_memcpy(x, t, sizeof(x));
     } else {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) x[i] = i < valid ? p[i] : (T)0.0f;
@@ -99,8 +104,8 @@ __device__ __forceinline__ void store_codes(uint8_t* p, const float (&v)[kPer]) 
 
 // blockDim = (tx, 256 / tx): tx threads along a row's groups of eight, the rest along rows.
 template <int FMT, typename T>
-__global__ __launch_bounds__(256) void k_mx_quantise(const T* X, int64_t ldx, int64_t N, int D, bool vec, uint8_t* codes,
-                                                     int64_t ldc, uint8_t* scales, int64_t lds) {
+__global__ __launch_bounds__(256) void k_mx_quantise(const T* X, int64_t ldx, int64_t N, int D, uint8_t* codes, int64_t ldc,
+                                                     uint8_t* scales, int64_t lds) {
     const int groups = mx_blocks(D) * 4;
     const int g = blockIdx.x * blockDim.x + threadIdx.x;
     if (g >= groups) return;                  // groups is a multiple of 4: the four threads of a block leave together
@@ -108,7 +113,7 @@ __global__ __launch_bounds__(256) void k_mx_quantise(const T* X, int64_t ldx, in
     const int valid = D - c0 < 0 ? 0 : (D - c0 < kPer ? D - c0 : kPer);
     for (int64_t n = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; n < N; n += (int64_t)gridDim.y * blockDim.y) {
         T x[kPer];
-        load8(X + n * ldx + c0, valid, vec, x);
+        load8(X + n * ldx + c0, valid, x);
         using M = typename std::conditional<sizeof(T) == 8, double, float>::type;
         auto a = mag_bits((M)x[0]);
 #pragma unroll
@@ -128,16 +133,16 @@ __global__ __launch_bounds__(256) void k_mx_quantise(const T* X, int64_t ldx, in
 }
 
 template <typename T>
-__device__ __forceinline__ void store8(T* p, int valid, bool vec, const float (&v)[kPer]) {
+__device__ __forceinline__ void store8(T* p, int valid, const float (&v)[kPer]) {
     T x[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) x[i] = (T)v[i];
-    if (vec && valid == kPer) {
+    if (valid == kPer) {
         constexpr int W = (int)sizeof(T) * kPer / 16;
-        u32x4 t[W];
-        __builtin_memcpy(t, x, sizeof(t));
+        typename Wide<T>::type t[W];
+        __builtin_memcpy(t, x, sizeof(x));
 #pragma unroll
-        for (int i = 0; i < W; ++i) ((u32x4*)p)[i] = t[i];
+        for (int i = 0; i < W; ++i) ((typename Wide<T>::type*)p)[i] = t[i];
     } else {
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
@@ -147,7 +152,7 @@ __device__ __forceinline__ void store8(T* p, int valid, bool vec, const float (&
 
 template <int FMT, typename T>
 __global__ __launch_bounds__(256) void k_mx_dequantise(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds,
-                                                       int64_t N, int D, bool vec, T* out, int64_t ldo) {
+                                                       int64_t N, int D, T* out, int64_t ldo) {
     const int g = blockIdx.x * blockDim.x + threadIdx.x;
     const int c0 = g * kPer;
     if (c0 >= D) return;
@@ -165,7 +170,7 @@ __global__ __launch_bounds__(256) void k_mx_dequantise(const uint8_t* codes, int
         } else {
             mx_word<FMT>(*(const unsigned*)(codes + n * ldc + (int64_t)g * 4), s, v);
         }
-        store8(out + n * ldo + c0, valid, vec, v);
+        store8(out + n * ldo + c0, valid, v);
     }
 }
 
@@ -183,8 +188,7 @@ template <int FMT, typename T>
 int quantise(const void* X, int64_t ldx, int64_t N, int D, void* codes, int64_t ldc, void* scales, int64_t lds, hipStream_t st) {
     dim3 grid, block;
     stream_shape(mx_blocks(D) * 4, N, grid, block);
-    const bool vec = (uintptr_t)X % 16 == 0 && ldx * (int64_t)sizeof(T) % 16 == 0;
-    hipLaunchKernelGGL((k_mx_quantise<FMT, T>), grid, block, 0, st, (const T*)X, ldx, N, D, vec, (uint8_t*)codes, ldc,
+    hipLaunchKernelGGL((k_mx_quantise<FMT, T>), grid, block, 0, st, (const T*)X, ldx, N, D, (uint8_t*)codes, ldc,
                        (uint8_t*)scales, lds);
     return vt_launch_status();
 }
@@ -194,9 +198,8 @@ int dequantise(const void* codes, int64_t ldc, const void* scales, int64_t lds, 
                hipStream_t st) {
     dim3 grid, block;
     stream_shape(mx_blocks(D) * 4, N, grid, block);
-    const bool vec = (uintptr_t)out % 16 == 0 && ldo * (int64_t)sizeof(T) % 16 == 0;
     hipLaunchKernelGGL((k_mx_dequantise<FMT, T>), grid, block, 0, st, (const uint8_t*)codes, ldc, (const uint8_t*)scales, lds,
-                       N, D, vec, (T*)out, ldo);
+                       N, D, (T*)out, ldo);
     return vt_launch_status();
 }
 

@@ -81,10 +81,7 @@ __device__ __forceinline__ double mx_row_op(const MxRows& a, int64_t n, const Ro
 typedef __amdgpu_buffer_rsrc_t MxRsrc;
 __device__ __forceinline__ MxRsrc rows_rsrc(const uint8_t* base, int64_t n0, int64_t ld, int64_t N, int64_t width) {
     const int64_t bytes = n0 < N ? (N - 1 - n0) * ld + width : 0;
-    const uint64_t p = (uint64_t)(base + n0 * ld);
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)p), hi = __builtin_amdgcn_readfirstlane((uint32_t)(p >> 32));
-    return __builtin_amdgcn_make_buffer_rsrc((void*)(((uint64_t)hi << 32) | lo), 0,
-                                             __builtin_amdgcn_readfirstlane((uint32_t)std::min<int64_t>(bytes, 0xfffffff0)), 0x00020000);
+    return mx_rsrc(base + n0 * ld, bytes);
 }
 
 template <int FMT> struct Piece;
