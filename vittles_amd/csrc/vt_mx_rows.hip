@@ -294,7 +294,7 @@ __global__ __launch_bounds__(T, 2) void k_mx_rows_wide(MxRows a) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int nb = mx_blocks(a.D), pieces = 2 * nb, own = lane / kLead;
     f64x2* const vl = (f64x2*)dyn;
-    double* const red = dyn + (kDot<OP> ? 16 * pieces : 0);       // [2][R][kWaves]
+    double* const red = dyn + 16 * pieces;       // [2][R][kWaves]
     const int last = pieces - (CPT - 1) * T;                      // pieces of the last round of threads, >= 1
     unsigned vc[CPT], vs[CPT];
     double acc[kCols<OP> ? CPT : 1][16];
@@ -308,13 +308,9 @@ __global__ __launch_bounds__(T, 2) void k_mx_rows_wide(MxRows a) {
         }
     }
     if constexpr (kDot<OP>) {
-#pragma unroll
-        for (int k = 0; k < CPT; ++k) {
-            const int width = k < CPT - 1 ? T : last, c = 16 * (tid + T * k);
-            if (tid < width)
-#pragma unroll
-                for (int p = 0; p < 8; ++p)
-                    vl[8 * T * k + p * width + tid] = f64x2{c + 2 * p < a.D ? a.v[c + 2 * p] : 0.0, c + 2 * p + 1 < a.D ? a.v[c + 2 * p + 1] : 0.0};
+        for (int i = tid; i < 8 * pieces; i += T) {          // pair i: piece i / 8, its pair i % 8
+            const int c = 2 * i, piece = i >> 3, k = piece / T, width = k < CPT - 1 ? T : last;
+            vl[8 * T * k + (i & 7) * width + piece - T * k] = f64x2{c < a.D ? a.v[c] : 0.0, c + 1 < a.D ? a.v[c + 1] : 0.0};
         }
         __syncthreads();
     }
@@ -419,14 +415,22 @@ __global__ __launch_bounds__(T, 2) void k_mx_rows_wide(MxRows a) {
         }
     }
     if constexpr (kCols<OP>) {
+        // through LDS, so that the slab is written in order (a lane's own 16 columns are 128 bytes apart); the pairs of a
+        // piece are turned by its number: other banks for every lane
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < CPT; ++k) {
+            const int piece = tid + T * k;
+            if (piece < pieces)
+#pragma unroll
+                for (int p = 0; p < 8; ++p) vl[8 * piece + (p ^ (piece & 7))] = f64x2{acc[k][2 * p], acc[k][2 * p + 1]};
+        }
+        __syncthreads();
         double* out = a.part + (int64_t)blockIdx.x * a.D;
-#pragma unroll
-        for (int k = 0; k < CPT; ++k)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int c = 16 * (tid + T * k) + e;
-                if (c < a.D) out[c] = acc[k][e];
-            }
+        for (int c = tid; c < a.D; c += T) {
+            const int piece = c >> 4;
+            out[c] = vl[8 * piece + ((c >> 1 & 7) ^ (piece & 7))][c & 1];
+        }
     }
     if constexpr (OP == OP_VALUE) {
         if (wave == 0) {
@@ -530,7 +534,7 @@ __global__ __launch_bounds__(1024) void k_mx_sum(const double* t, int64_t N, dou
     }
 }
 
-// Which kernel takes a width: 2, 8, 32 or 64 lanes of a wave (D <= 1024), a workgroup of 128, 256 or 512 threads with one
+// Which kernel takes a width: 2 to 64 lanes of a wave (D <= 1024), a workgroup of 128, 256 or 512 threads with one
 // piece each (D <= 8192: fewer threads with more pieces were slower, D = 4096: 112 us in 256 x 1, 143 in 128 x 2), 512 with
 // two or three, else two passes.  v and the sums of a round share 160 KB of LDS: D <= 20352 in one pass.
 constexpr int kOnePassPieces = (160 * 1024 - 1024) / 128;
@@ -556,7 +560,7 @@ RowsPlan rows_plan(int format, int64_t N, int D, int64_t ldc, int64_t lds) {
     // (offsets inside a round are 32 bits: 256 rows at most)
     const bool far = ldc >= 1 << 22 || lds >= 1 << 22;
     if (pieces <= 64 && !far) {
-        p.lanes = pieces <= 2 ? 2 : pieces <= 8 ? 8 : pieces <= 32 ? 32 : 64;
+        for (p.lanes = 2; p.lanes < pieces;) p.lanes *= 2;
         const int rows = 256 / p.lanes * wave_rows(p.lanes);
         rounds = (N + rows - 1) / rows, most = 2 * cu;
     } else if (pieces <= kOnePassPieces && !far) {
@@ -584,7 +588,7 @@ template <int OP, int FMT, int T, int CPT>
 int launch_wide(const MxRows& a, int grid, hipStream_t st) {
     constexpr bool keep = CPT == 1;
     constexpr int R = wide_rows(CPT, FMT);
-    const size_t lds = (kDot<OP> ? 128 * (size_t)(2 * mx_blocks(a.D)) : 0) + 2 * (T / 64) * R * sizeof(double);
+    const size_t lds = 128 * (size_t)(2 * mx_blocks(a.D)) + 2 * (T / 64) * R * sizeof(double);
     static VtLdsAttr attr;
     if (vt_allow_big_lds((const void*)k_mx_rows_wide<OP, FMT, T, CPT, R, keep>, attr, 160 * 1024) != VT_OK) return VT_ERR_HIP;
     hipLaunchKernelGGL((k_mx_rows_wide<OP, FMT, T, CPT, R, keep>), dim3(grid), dim3(T), lds, st, a);
@@ -596,7 +600,9 @@ int run(MxRows a, const RowsPlan& p, hipStream_t st) {
     if (p.lanes > 0) {
         switch (p.lanes) {
             case 2: launch_wave<OP, FMT, 2>(a, p.grid, st); break;
+            case 4: launch_wave<OP, FMT, 4>(a, p.grid, st); break;
             case 8: launch_wave<OP, FMT, 8>(a, p.grid, st); break;
+            case 16: launch_wave<OP, FMT, 16>(a, p.grid, st); break;
             case 32: launch_wave<OP, FMT, 32>(a, p.grid, st); break;
             default: launch_wave<OP, FMT, 64>(a, p.grid, st); break;
         }
