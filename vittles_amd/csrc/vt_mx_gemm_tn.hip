@@ -108,7 +108,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tn(MxTN a, int tiles_d, 
         const int64_t left = n_hi - n0;
         const auto ra = mx_rsrc(a.codes + n0 * a.ldc, left > 0 ? (left - 1) * a.ldc + (FMT == VT_MX_FP8 ? width : width / 2) : 0);
         const auto rs = mx_rsrc(a.scales + n0 * a.lds, left > 0 ? (left - 1) * a.lds + width / kMxBlock : 0);
-        const int64_t last = VEC ? (a.Db + 7) / 8 * 8 : a.Db;
+        constexpr int kWide = 16 / sizeof(T);        // a load that holds a row's last column ends inside its 16 bytes
+        const int64_t last = (a.Db + kWide - 1) / kWide * kWide;
         const auto rb = mx_rsrc((const T*)a.B + n0 * a.ldb, left > 0 ? ((left - 1) * a.ldb + last) * (int64_t)sizeof(T) : 0);
 #pragma unroll
         for (int i = 0; i < S::kLoadsA; ++i) {
@@ -375,6 +376,7 @@ extern "C" int vt_mx_gemm_tn(int format, const void* codes, int64_t ldc, const v
     if (type < VT_TYPE_F32 || type > VT_TYPE_F16 || (N > 0 && (!B || ldb < Db))) return VT_ERR_BAD_ARG;
     const TnPlan p = plan(N, Da, Db);
     if (!ws || ws_bytes < vt_mx_gemm_tn_workspace_bytes(N, Da, Db)) return VT_ERR_WORKSPACE;
+    if (N <= 1) ldb = (Db + 7) / 8 * 8;      // a single row has no stride
     // 32-bit offsets inside a chunk of 64 rows, tile numbers in 31 bits
     if (ldc >= 1 << 25 || lds >= 1 << 25 || (N > 1 && ldb >= 1 << 23) || ldo >= 1 << 24) return VT_ERR_UNSUPPORTED;
     if ((int64_t)((Da + p.bm - 1) / p.bm) * ((Db + p.bn - 1) / p.bn) * p.slabs > 0x7ffffff0) return VT_ERR_UNSUPPORTED;

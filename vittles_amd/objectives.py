@@ -108,7 +108,7 @@ class WeightedGLMObjective(RegisteredObjective):
         if isinstance(X, compact.CompactRows):
             if dtype not in (torch.float64, X.format):          # torch.float64: the default, not asked for
                 raise ValueError("X is stored in %s already: dtype cannot be %s" % (X.format, dtype))
-            if device is not None and torch.device(device) != X.device:
+            if device is not None and torch.device(device) not in (X.device, torch.device(X.device.type)):
                 raise ValueError("X is on %s already" % X.device)
             dtype = X.format
         if dtype not in (torch.float64, torch.float32) + compact.FORMATS:

@@ -306,6 +306,8 @@ def gemm_tn_tiled(A, B, tile=8192):
     into column panels and every (panel of A, panel of B) pair is one vt_gemm_tn call into its slice of the result
     (no library GEMM on the path)."""
     Da, Db = A.shape[1], B.shape[1]
+    if isinstance(A, CompactRows):          # of any width as it is
+        return gemm_tn(A, B)
     if Da <= tile and Db <= tile and Da >= 1 and Db >= 1:
         return gemm_tn(A, B)
     out = torch.empty((Da, Db), dtype=torch.float64, device=A.device)
