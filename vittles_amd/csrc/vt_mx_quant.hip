@@ -132,49 +132,58 @@ __global__ __launch_bounds__(256) void k_mx_quantise(const T* X, int64_t ldx, in
     }
 }
 
-template <typename T>
-__device__ __forceinline__ void store8(T* p, int valid, const float (&v)[kPer]) {
-    T x[kPer];
+template <int PER, typename T>
+__device__ __forceinline__ void store_per(T* p, int valid, const float (&v)[PER]) {
+    T x[PER];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) x[i] = (T)v[i];
-    if (valid == kPer) {
-        constexpr int W = (int)sizeof(T) * kPer / 16;
+    for (int i = 0; i < PER; ++i) x[i] = (T)v[i];
+    if (valid == PER) {
+        constexpr int W = (int)sizeof(T) * PER / 16;
         typename Wide<T>::type t[W];
         __builtin_memcpy(t, x, sizeof(x));
 #pragma unroll
         for (int i = 0; i < W; ++i) ((typename Wide<T>::type*)p)[i] = t[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i)
+        for (int i = 0; i < PER; ++i)
             if (i < valid) p[i] = x[i];
     }
 }
 
+// Columns a thread reads back.  Eight of a double would be four stores 64 bytes apart between lanes; with two a wave's
+// store is one run (65536 x 4096 from E4M3: 663 -> 483 us).
+template <typename T> constexpr int kBack = sizeof(T) == 8 ? 2 : 8;
+
 template <int FMT, typename T>
 __global__ __launch_bounds__(256) void k_mx_dequantise(const uint8_t* codes, int64_t ldc, const uint8_t* scales, int64_t lds,
                                                        int64_t N, int D, T* out, int64_t ldo) {
+    constexpr int P = kBack<T>;
     const int g = blockIdx.x * blockDim.x + threadIdx.x;
-    const int c0 = g * kPer;
+    const int c0 = g * P;
     if (c0 >= D) return;
-    const int valid = D - c0 < kPer ? D - c0 : kPer;
+    const int valid = D - c0 < P ? D - c0 : P;
     for (int64_t n = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; n < N; n += (int64_t)gridDim.y * blockDim.y) {
-        const float s = mx_scale(scales[n * lds + (g >> 2)]);
-        float v[kPer];
-        if constexpr (FMT == VT_MX_FP8) {
-            const u32x2 w = *(const u32x2*)(codes + n * ldc + (int64_t)g * 8);
+        const float s = mx_scale(scales[n * lds + c0 / kMxBlock]);
+        const uint8_t* p = codes + n * ldc + (FMT == VT_MX_FP8 ? c0 : c0 / 2);
+        float v[P];
+        if constexpr (P == 2) {
+            const f32x2 t = mx_pair<FMT, 0>(FMT == VT_MX_FP8 ? (unsigned)*(const uint16_t*)p : (unsigned)*p, s);
+            v[0] = t[0], v[1] = t[1];
+        } else if constexpr (FMT == VT_MX_FP8) {
+            const u32x2 w = *(const u32x2*)p;
             float t[4];
             mx_word<FMT>(w[0], s, t);
             v[0] = t[0], v[1] = t[1], v[2] = t[2], v[3] = t[3];
             mx_word<FMT>(w[1], s, t);
             v[4] = t[0], v[5] = t[1], v[6] = t[2], v[7] = t[3];
         } else {
-            mx_word<FMT>(*(const unsigned*)(codes + n * ldc + (int64_t)g * 4), s, v);
+            mx_word<FMT>(*(const unsigned*)p, s, v);
         }
-        store8(out + n * ldo + c0, valid, v);
+        store_per<P>(out + n * ldo + c0, valid, v);
     }
 }
 
-// Threads along the row: the power of two that covers its groups of eight, 256 at most.
+// Threads along the row: the power of two that covers its groups of columns, 256 at most.
 void stream_shape(int groups, int64_t N, dim3& grid, dim3& block) {
     int tx = 4;
     while (tx < groups && tx < 256) tx *= 2;
@@ -197,7 +206,7 @@ template <int FMT, typename T>
 int dequantise(const void* codes, int64_t ldc, const void* scales, int64_t lds, int64_t N, int D, void* out, int64_t ldo,
                hipStream_t st) {
     dim3 grid, block;
-    stream_shape(mx_blocks(D) * 4, N, grid, block);
+    stream_shape(D / kBack<T> + (D % kBack<T> != 0), N, grid, block);
     hipLaunchKernelGGL((k_mx_dequantise<FMT, T>), grid, block, 0, st, (const uint8_t*)codes, ldc, (const uint8_t*)scales, lds,
                        N, D, (T*)out, ldo);
     return vt_launch_status();
