@@ -39,8 +39,8 @@ __device__ __forceinline__ void mx_store(const MxNT& a, int64_t m, int64_t n, fl
 // (LDS-DMA, 16 bytes a lane for codes, 4 for scales) while this one is multiplied.
 // LDS: 16-byte slot j of row r holds block j ^ ((r >> 1) & 7), so the sixteen rows that are read at a time lie in
 // different banks.  The DMA writes slots in lane order; the permutation is in the lanes' addresses.
-// Measured at 8192^3: 320 - 335 us = 3.3 - 3.4 PFLOP/s.  Of these the codes' way from L2 alone takes 225 (2.1 GB at the
-// ~10 TB/s that two chunks in flight draw), products and operand reads alone 214, writing C 50: the first two overlap,
+// Measured at 8192^3: 296 us = 3.7 PFLOP/s (4096^2 x 8192: 79 us, 3.5).  The codes' way from L2 alone takes 225 (2.1 GB at
+// the ~10 TB/s that two chunks in flight draw), products and operand reads alone 214, writing C 50: the first two overlap,
 // the last does not, a tile's workgroup fills its CU.  Reading operands a step ahead, with the barrier under the last
 // step's products, took the same time.
 constexpr int kChunk = 8, kRow = 16 * kChunk, kRowsPerLoad = 1024 / kRow;
@@ -238,7 +238,7 @@ __global__ __launch_bounds__(256) void k_mx_nt_join(MxNT a, int slices) {
 // Blocks of at most 16 MT rows of the shorter side ("few", F): each workgroup streams 16 rows of the other side ("many")
 // straight from memory into v_mfma_scale_f32_16x16x128, its four waves on interleaved chunks of the axis, joined through
 // LDS.  For up to 64 rows reading the many rows once is the whole cost; for small products with more it saves the tiles'
-// long way in and out (151 x 219 x 563: 13.5 us in tiles).  SWAP: the few rows are B's.
+// long way in and out (151 x 219 x 563: 6.3 us, 13.5 in tiles).  SWAP: the few rows are B's.
 struct MxFew {
     const uint8_t *cm, *sm, *cf, *sf;      // many, few
     int64_t ldcm, ldsm, ldcf, ldsf, many, few;
@@ -335,17 +335,19 @@ NtPlan plan(int64_t M, int64_t N, int K, bool far) {
         p.few = less <= 64 ? (int)((less + 15) / 16) : 4;
         return p;
     }
-    // Tiles: 256 x 256, one to a CU, or 128 x 128, two.  A round of them took about 18 + 2 us a chunk in the first (4096^2 and
-    // 8192^2, 256 to 8192 columns), 12 + 1.3 in the second; it says 47 against 33 us at 2048 x 4096 x 4096 and 82 against
-    // 107 at 4096 x 4096 x 8192, measured 47, 33, 82 and 105.
+    // Tiles: 256 x 256, one to a CU: every round takes 17 + 1.75 us a chunk, the writing of C hides behind nothing.
+    // 128 x 128, two to a CU: 6 us once and 5 + 1.2 a chunk for a round, one writes while the other multiplies.  Measured, us
+    // (256 / 128): 4096^2 x 4096 46 / 53, 8192^2 x 8192 299 / 359, x 2048 118 / 120, x 256 77 / 56, 6000^2 x 1024 47 / 43,
+    // 2048 x 4096 x 4096 34 / 29, 3000 x 4000 x 2048 24 / 26.  Tiles of 256 x 128, one
+    // to a CU, were no better anywhere: 4096^2 x 4096 59, 8192^3 379, 2048 x 4096 x 4096 30.
     const int cu = vt_num_cu();
     const int chunks = (nb + kChunk - 1) / kChunk;
     const int64_t t = tiles(M, N, 128, 128);
-    const double big = (double)((tiles(M, N, 256, 256) + cu - 1) / cu) * (18.0 + 2.0 * chunks);
-    const double small = (double)((t + 2 * cu - 1) / (2 * cu)) * (12.0 + 1.3 * chunks);
+    const double big = (double)((tiles(M, N, 256, 256) + cu - 1) / cu) * (17.0 + 1.75 * chunks);
+    const double small = 6.0 + (double)((t + 2 * cu - 1) / (2 * cu)) * (5.0 + 1.2 * chunks);
     p.shape = big < small ? 0 : 1;
-    // few tiles and a long axis: slices of at least 8 chunks, joined by a second pass (300 x 300 x 8192: 32 us whole, 20
-    // in four slices; 512 x 4096 x 4096, 128 tiles: 23 us whole, 27 in two)
+    // few tiles and a long axis: slices of at least 8 chunks, joined by a second pass (512 x 512 x 8192: 24 us whole, 14
+    // in four slices; 512 x 4096 x 4096, 128 tiles: two slices took 4 us more than the whole)
     const int s = p.shape == 0 ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(cu / (2 * t), chunks / 8), 16));
     p.step = (chunks + s - 1) / s * kChunk;
     p.slices = (nb + p.step - 1) / p.step;

@@ -6,6 +6,10 @@
 // Both operands are contracted along the rows, across which they lie in memory: a chunk of rows is staged as it lies and
 // read with the transposing LDS read (ds_read_b64_tr_b16), 4 rows x 16 columns a quarter wave.
 // The long axis N is cut into slabs; a slab's sums are float and the slabs are added in a fixed order.
+// Bound: the matrix unit, once a part: 8192 x 4096 x 4096 takes 235 us in bfloat16 (1.17 PFLOP/s), 461 in half and 667 in
+// float or weighted.  What keeps it from the 1.5 of a large product is the codes' way through registers (conversion and
+// LDS writes, about 4 VALU instructions an MFMA); where the slabs' sums are large, also their way out and back
+// (16384 x 4096 x 1000: 150 us, about 30 of them).
 #include "vt_mx.h"
 #include <type_traits>
 
@@ -311,7 +315,7 @@ struct TnPlan {
 TnPlan plan(int64_t N, int Da, int Db) {
     TnPlan p;
     // 128 x 64 tiles where a round or two of them with 128 rows each is the whole product: the way in and out of a tile of
-    // 256 x 256 alone takes longer
+    // 256 x 256 alone takes longer (35 x 1156 x 217 in float: 7 us, 28 in tiles of 256 x 256)
     const int64_t small = (int64_t)((Da + 127) / 128) * ((Db + 63) / 64) * ((N + 127) / 128);
     if (Db <= 64 || small <= 4 * vt_num_cu()) p.bm = 128, p.bn = 64;
     else p.bm = 256, p.bn = Db > 128 ? 256 : 128;

@@ -5,8 +5,8 @@
 // whole kernel.  Partial sums are combined in a fixed order (no atomics: the same bits every time).
 // Bound: HBM for E4M3 (reads alone: 5.4 - 5.9 TB/s), the VALU for E2M1.  An element costs half a conversion to float and
 // one to double, once if its double is kept and twice if not, and two fp64 FMAs: 3.5 to 5 instructions of 4 cycles for 64
-// elements, and about 100 more a round for the sums.  Measured, HVP in TB/s of stored bytes: E4M3 N = 4 10^6, D = 100 5.1;
-// N = 10^5, D = 8192 4.8, D = 20 000 4.1 (503 us); E2M1 3.2, 2.6, 2.6 (405 us).
+// elements, and about 100 more a round for the sums.  Measured, HVP in TB/s of stored bytes: E4M3 N = 4 10^6, D = 100 4.6;
+// N = 10^5, D = 8192 4.6, D = 20 000 4.4 (474 us); E2M1 3.1, 2.8, 2.7 (391 us); A v 5.9 and 4.2 at most.
 #include "vt_mx.h"
 #include <type_traits>
 #include <utility>
@@ -545,8 +545,8 @@ struct RowsPlan {
 };
 
 // Rows a round.  One piece a thread: 4, kept as doubles (128 registers).  Two pieces: 4, decoded twice (N = 50 000,
-// D = 16 384: 206 us; 2 kept rows 222).  Three pieces: 4 fit for E2M1; for E4M3 2 (N = 100 000, D = 20 000: 503 us; 4 spill:
-// 985).
+// D = 16 384: 206 us; 2 kept rows 222).  Three pieces: 4 fit for E2M1; for E4M3 2 (N = 100 000, D = 20 000: 474 us; 4 spill:
+// 985).  Of one piece, two rows a round with more waves resident: 20 to 40 % longer; a round's time is what the VALU issues.
 constexpr int wave_rows(int lanes) { return lanes < 4 ? lanes : 4; }
 constexpr int wide_rows(int cpt, int format) { return cpt == 3 && format == VT_MX_FP8 ? 2 : 4; }
 
