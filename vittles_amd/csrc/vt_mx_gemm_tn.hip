@@ -6,10 +6,11 @@
 // Both operands are contracted along the rows, across which they lie in memory: a chunk of rows is staged as it lies and
 // read with the transposing LDS read (ds_read_b64_tr_b16), 4 rows x 16 columns a quarter wave.
 // The long axis N is cut into slabs; a slab's sums are float and the slabs are added in a fixed order.
-// Bound: the matrix unit, once a part: 8192 x 4096 x 4096 takes 235 us in bfloat16 (1.17 PFLOP/s), 461 in half and 667 in
-// float or weighted.  What keeps it from the 1.5 of a large product is the codes' way through registers (conversion and
-// LDS writes, about 4 VALU instructions an MFMA); where the slabs' sums are large, also their way out and back
-// (16384 x 4096 x 1000: 150 us, about 30 of them).
+// Bound: the matrix unit, once a part: 8192 x 4096 x 4096 takes 240 us in bfloat16 (1.15 PFLOP/s; a library product of
+// 8192^3 reaches 1.36), 470 in half, 680 in float and 725 weighted.  Two VALU instructions go with an MFMA (conversion, the
+// way to LDS); reading operands a step ahead, spreading the writes to LDS over the steps, or fixing the order of the two
+// took the same time within 2 %, one chunk ahead instead of two 8 to 18 % longer.  Where the slabs' sums are large, their
+// way out and back counts too (16384 x 4096 x 1000: 15 of 155 us).
 #include "vt_mx.h"
 #include <type_traits>
 
