@@ -9,12 +9,19 @@ import torch
 from . import _lib
 
 
+_found = None       # the library, once a device has been seen (0.8 us a call to ask again)
+
+
 def require_gpu():
     """Fail loudly when the HIP path cannot run (no silent CPU fallback)."""
+    global _found
+    if _found is not None:
+        return _found
     lib = _lib.load()
     if not torch.cuda.is_available() or lib.vt_device_count() <= 0:
         raise _lib.VittlesHipError(
             "vittles_amd needs an AMD GPU (gfx950): no HIP device is visible and there is no CPU fallback.")
+    _found = lib
     return lib
 
 
