@@ -285,10 +285,14 @@ __global__ __launch_bounds__(256, 2) void k_mx_rows_wave(MxRows a) {
 // rows), the column sums in registers, one barrier a round for the dots.  v's pairs lie [piece / T][pair][piece % T] so
 // that the lanes of a read are next to each other.  KEEP: the round's numbers stay in registers as doubles (16 CPT R of
 // them) from the dot to the column sums; else the codes are decoded twice.
-template <int OP, int FMT, int T, int CPT, int R, bool KEEP>
-__global__ __launch_bounds__(T, 2) void k_mx_rows_wide(MxRows a) {
+// TEAM = 0, for the operators without column sums: exactly the waves that a row needs, and more of them resident (A v
+// N = 100 000, D = 5003, E2M1: 123 -> 78 us; with column sums that costs 10 to 30 %).
+constexpr int few_waves(int op) { return op == OP_VALUE ? 3 : 4; }       // of a SIMD (a fourth of VALUE's would spill)
+template <int OP, int FMT, int TEAM, int CPT, int R, bool KEEP>
+__global__ __launch_bounds__(TEAM ? TEAM : 512, TEAM ? 2 : few_waves(OP)) void k_mx_rows_wide(MxRows a) {
     using W = typename Piece<FMT>::type;
-    constexpr int kBytes = sizeof(W), kWaves = T / 64, kLead = 64 / R;
+    constexpr int kBytes = sizeof(W), kWaves = TEAM ? TEAM / 64 : 8, kLead = 64 / R;
+    const int T = TEAM ? TEAM : blockDim.x;
     static_assert(kWaves <= kLead, "a row's wave sums fit its lanes");
     extern __shared__ __align__(16) double dyn[];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -378,7 +382,7 @@ __global__ __launch_bounds__(T, 2) void k_mx_rows_wide(MxRows a) {
             double* const slot = red + (it & 1) * kWaves * R + own * kWaves;
             if (lane % kLead == 0) slot[wave] = mine;
             vt_lds_barrier();
-            const double part[1] = {slot[lane & (kWaves - 1)]};
+            const double part[1] = {TEAM || (lane & (kWaves - 1)) < T / 64 ? slot[lane & (kWaves - 1)] : 0.0};
             dot = team_sum<kWaves, 1>(part, lane);
         }
         const int64_t n = n0 + own;
@@ -552,7 +556,8 @@ constexpr int wide_rows(int cpt, int format) { return cpt == 3 && format == VT_M
 
 int col_tiles(int D) { return (D + 2047) / 2048; }
 
-RowsPlan rows_plan(int format, int64_t N, int D, int64_t ldc, int64_t lds) {
+// `op`: an operator with column sums unless said otherwise (those without may have more workgroups, and need no slabs)
+RowsPlan rows_plan(int format, int64_t N, int D, int64_t ldc, int64_t lds, int op = OP_GRAD) {
     const int pieces = 2 * mx_blocks(D), cu = vt_num_cu();
     RowsPlan p{0, 0, 0, 0};
     int64_t rounds;               // of all workgroups together
@@ -568,7 +573,9 @@ RowsPlan rows_plan(int format, int64_t N, int D, int64_t ldc, int64_t lds) {
         p.cpt = (pieces + p.threads - 1) / p.threads;
         const int rows = wide_rows(p.cpt, format);
         rounds = (N + rows - 1) / rows;
-        most = cu * std::max(1, std::min(512 / p.threads, (160 * 1024) / (128 * pieces + 1024)));
+        int waves = 8;                // of a CU
+        if (p.cpt == 1 && (op == OP_LINK || op == OP_VALUE || op == OP_GEMV)) p.threads = (pieces + 63) / 64 * 64, waves = 4 * few_waves(op);
+        most = cu * std::max(1, std::min(64 * waves / p.threads, (160 * 1024) / (128 * pieces + 1024)));
     } else {
         p.grid = (int)std::max<int64_t>(1, std::min<int64_t>(N, std::max(1, 4 * cu / col_tiles(D))));
         return p;
@@ -585,13 +592,13 @@ void launch_wave(const MxRows& a, int grid, hipStream_t st) {
 }
 
 template <int OP, int FMT, int T, int CPT>
-int launch_wide(const MxRows& a, int grid, hipStream_t st) {
-    constexpr bool keep = CPT == 1;
+int launch_wide(const MxRows& a, const RowsPlan& p, hipStream_t st) {
+    constexpr bool keep = kCols<OP> && CPT == 1;
     constexpr int R = wide_rows(CPT, FMT);
-    const size_t lds = 128 * (size_t)(2 * mx_blocks(a.D)) + 2 * (T / 64) * R * sizeof(double);
+    const size_t lds = 128 * (size_t)(2 * mx_blocks(a.D)) + 2 * (T ? T / 64 : 8) * R * sizeof(double);
     static VtLdsAttr attr;
     if (vt_allow_big_lds((const void*)k_mx_rows_wide<OP, FMT, T, CPT, R, keep>, attr, 160 * 1024) != VT_OK) return VT_ERR_HIP;
-    hipLaunchKernelGGL((k_mx_rows_wide<OP, FMT, T, CPT, R, keep>), dim3(grid), dim3(T), lds, st, a);
+    hipLaunchKernelGGL((k_mx_rows_wide<OP, FMT, T, CPT, R, keep>), dim3(p.grid), dim3(p.threads), lds, st, a);
     return VT_OK;
 }
 
@@ -609,11 +616,13 @@ int run(MxRows a, const RowsPlan& p, hipStream_t st) {
         return vt_launch_status();
     }
     if (p.threads > 0) {
-        const int rc = p.threads == 128   ? launch_wide<OP, FMT, 128, 1>(a, p.grid, st)
-                       : p.threads == 256 ? launch_wide<OP, FMT, 256, 1>(a, p.grid, st)
-                       : p.cpt == 1       ? launch_wide<OP, FMT, 512, 1>(a, p.grid, st)
-                       : p.cpt == 2       ? launch_wide<OP, FMT, 512, 2>(a, p.grid, st)
-                                          : launch_wide<OP, FMT, 512, 3>(a, p.grid, st);
+        int rc;
+        if (p.cpt == 3) rc = launch_wide<OP, FMT, 512, 3>(a, p, st);
+        else if (p.cpt == 2) rc = launch_wide<OP, FMT, 512, 2>(a, p, st);
+        else if constexpr (!kCols<OP>) rc = launch_wide<OP, FMT, 0, 1>(a, p, st);
+        else rc = p.threads == 128   ? launch_wide<OP, FMT, 128, 1>(a, p, st)
+                  : p.threads == 256 ? launch_wide<OP, FMT, 256, 1>(a, p, st)
+                                     : launch_wide<OP, FMT, 512, 1>(a, p, st);
         return rc != VT_OK ? rc : vt_launch_status();
     }
     const int grid = (int)std::min<int64_t>((a.N + 3) / 4, 8 * (int64_t)vt_num_cu());
@@ -657,17 +666,17 @@ extern "C" size_t vt_mx_rows_workspace_bytes(int64_t N, int D) {
     return ws_doubles(N, D) * sizeof(double);
 }
 
-#define VT_MX_ROWS_PROLOGUE                                                                  \
+#define VT_MX_ROWS_PROLOGUE(op)                                                              \
     if (!mx_rows_ok(format, codes, ldc, scales, lds, N, D)) return VT_ERR_BAD_ARG;           \
     if (!ws || ws_bytes < vt_mx_rows_workspace_bytes(N, D)) return VT_ERR_WORKSPACE;         \
     hipStream_t st = (hipStream_t)stream;                                                    \
-    const RowsPlan p = rows_plan(format, N, D, ldc, lds);                                        \
+    const RowsPlan p = rows_plan(format, N, D, ldc, lds, op);                                \
     MxRows a = rows_of(codes, ldc, scales, lds, N, D, ws, p);
 
 extern "C" int vt_mx_glm_link(int family, int format, const void* codes, int64_t ldc, const void* scales, int64_t lds,
                               const double* theta, const double* y, const double* w, const double* offset, double scale,
                               int64_t N, int D, double* z, double* r, double* d, void* ws, size_t ws_bytes, void* stream) {
-    VT_MX_ROWS_PROLOGUE
+    VT_MX_ROWS_PROLOGUE(OP_LINK)
     if (family < 0 || family > 2) return VT_ERR_BAD_ARG;
     if (N == 0) return VT_OK;
     if (!theta || !y || !w) return VT_ERR_BAD_ARG;
@@ -680,7 +689,7 @@ extern "C" int vt_mx_glm_grad(int family, int format, const void* codes, int64_t
                               const double* theta, const double* y, const double* w, const double* offset, double scale,
                               const double* prior, int64_t N, int D, double* g, double* r, double* d, void* ws,
                               size_t ws_bytes, void* stream) {
-    VT_MX_ROWS_PROLOGUE
+    VT_MX_ROWS_PROLOGUE(OP_GRAD)
     if (family < 0 || family > 2 || !theta || !g || (N > 0 && (!y || !w))) return VT_ERR_BAD_ARG;
     a.v = theta, a.y = y, a.w = w, a.offset = offset, a.scale = scale, a.family = family, a.r = r, a.d = d;
     if (N > 0)
@@ -691,7 +700,7 @@ extern "C" int vt_mx_glm_grad(int family, int format, const void* codes, int64_t
 extern "C" int vt_mx_glm_value(int family, int format, const void* codes, int64_t ldc, const void* scales, int64_t lds,
                                const double* theta, const double* y, const double* w, const double* offset, double scale,
                                int64_t N, int D, double* value, void* ws, size_t ws_bytes, void* stream) {
-    VT_MX_ROWS_PROLOGUE
+    VT_MX_ROWS_PROLOGUE(OP_VALUE)
     if (family < 0 || family > 2 || !theta || !value || (N > 0 && (!y || !w))) return VT_ERR_BAD_ARG;
     a.v = theta, a.y = y, a.w = w, a.offset = offset, a.family = family;
     if (N > 0)
@@ -704,7 +713,7 @@ extern "C" int vt_mx_glm_value(int family, int format, const void* codes, int64_
 extern "C" int vt_mx_glm_hvp(int format, const void* codes, int64_t ldc, const void* scales, int64_t lds, const double* d,
                              const double* prior, double prior_scalar, const double* v, int64_t N, int D, double* out,
                              void* ws, size_t ws_bytes, void* stream) {
-    VT_MX_ROWS_PROLOGUE
+    VT_MX_ROWS_PROLOGUE(OP_HVP)
     if (!v || !out || (N > 0 && !d)) return VT_ERR_BAD_ARG;
     a.v = v, a.y = d;
     if (N > 0)
@@ -714,7 +723,7 @@ extern "C" int vt_mx_glm_hvp(int format, const void* codes, int64_t ldc, const v
 
 extern "C" int vt_mx_gemv(int format, const void* codes, int64_t ldc, const void* scales, int64_t lds, const double* v,
                           int64_t N, int D, double* out, void* ws, size_t ws_bytes, void* stream) {
-    VT_MX_ROWS_PROLOGUE
+    VT_MX_ROWS_PROLOGUE(OP_GEMV)
     if (N == 0) return VT_OK;
     if (!v || !out) return VT_ERR_BAD_ARG;
     a.v = v, a.z = out, a.t = nullptr;
@@ -723,7 +732,7 @@ extern "C" int vt_mx_gemv(int format, const void* codes, int64_t ldc, const void
 
 extern "C" int vt_mx_gemv_t(int format, const void* codes, int64_t ldc, const void* scales, int64_t lds, const double* u1,
                             const double* u2, int64_t N, int D, double* out, void* ws, size_t ws_bytes, void* stream) {
-    VT_MX_ROWS_PROLOGUE
+    VT_MX_ROWS_PROLOGUE(OP_GEMVT)
     if (!out || (N > 0 && !u1)) return VT_ERR_BAD_ARG;
     a.y = u1, a.w = u2;
     if (N > 0)
