@@ -319,6 +319,7 @@ __global__ __launch_bounds__(TEAM ? TEAM : 512, TEAM ? 2 : few_waves(OP)) void k
         __syncthreads();
     }
     double val = 0.0;
+    int turn = 0;                // without column sums: the wave whose turn it is to finish the round's rows
     W next[R][CPT];
     unsigned next_s[R][CPT];
     RowScal next_r;
@@ -382,13 +383,16 @@ __global__ __launch_bounds__(TEAM ? TEAM : 512, TEAM ? 2 : few_waves(OP)) void k
             double* const slot = red + (it & 1) * kWaves * R + own * kWaves;
             if (lane % kLead == 0) slot[wave] = mine;
             vt_lds_barrier();
-            const double part[1] = {TEAM || (lane & (kWaves - 1)) < T / 64 ? slot[lane & (kWaves - 1)] : 0.0};
-            dot = team_sum<kWaves, 1>(part, lane);
+            if (kCols<OP> || wave == turn) {
+                const double part[1] = {TEAM || (lane & (kWaves - 1)) < T / 64 ? slot[lane & (kWaves - 1)] : 0.0};
+                dot = team_sum<kWaves, 1>(part, lane);
+            }
         }
         const int64_t n = n0 + own;
         double t = 0.0;
-        if (n < a.N) t = mx_row_op<OP>(a, n, scal, dot, wave == 0 && lane % kLead == 0);
-        if constexpr (OP == OP_VALUE) val += wave == 0 && lane % kLead == 0 ? t : 0.0;
+        if (n < a.N && (kCols<OP> || wave == turn)) t = mx_row_op<OP>(a, n, scal, dot, (!kCols<OP> || wave == 0) && lane % kLead == 0);
+        if constexpr (OP == OP_VALUE) val += lane % kLead == 0 ? t : 0.0;
+        if constexpr (!kCols<OP>) turn = turn + 1 < T / 64 ? turn + 1 : 0;
         if constexpr (kCols<OP>) {
             double tr[R];
 #pragma unroll
@@ -437,9 +441,13 @@ __global__ __launch_bounds__(TEAM ? TEAM : 512, TEAM ? 2 : few_waves(OP)) void k
         }
     }
     if constexpr (OP == OP_VALUE) {
-        if (wave == 0) {
-            val = vt_sum64(val);
-            if (lane == 0) a.part[blockIdx.x] = val;
+        val = vt_sum64(val);
+        __syncthreads();
+        if (lane == 0) red[wave] = val;
+        __syncthreads();
+        if (tid == 0) {
+            for (int i = 1; i < T / 64; ++i) val += red[i];
+            a.part[blockIdx.x] = val;
         }
     }
 }
