@@ -8,11 +8,11 @@
 // The long axis N is cut into slabs; a slab's sums are float and the slabs are added in a fixed order.
 // Bound: the matrix unit, once a part: 8192 x 4096 x 4096 takes 240 us in bfloat16 (1.15 PFLOP/s; a library product of
 // 8192^3 reaches 1.36), 470 in half, 680 in float and 725 weighted.  Two VALU instructions go with an MFMA (conversion, the
-// way to LDS); reading operands a step ahead, spreading the writes to LDS over the steps, or fixing the order of the two
-// took the same time within 2 %; so did eight rows
-// of a column side by side in LDS, read with ds_read_b128 at twice the rate of the transposing read (133 against 72 bytes a
-// cycle) and shuffled into place by v_perm (3 to 8 % longer); one chunk ahead instead of two: 8 to 18 % longer.  Where the slabs' sums are large, their
-// way out and back counts too (16384 x 4096 x 1000: 15 of 155 us).
+// way to LDS).  Reading operands a step ahead, spreading the writes to LDS over the steps, or fixing the order of the two
+// took the same time within 2 %; eight rows of a column side by side in LDS, read with ds_read_b128 at twice the rate of
+// the transposing read (133 against 72 bytes a cycle) and put there by v_perm, 3 to 8 % longer; one chunk ahead instead of
+// two 8 to 18 % longer.  Where the slabs' sums are large, their way out and back counts too (16384 x 4096 x 1000: 15 of
+// 155 us).
 #include "vt_mx.h"
 #include <type_traits>
 

@@ -7,6 +7,7 @@
 // one to double, once if its double is kept and twice if not, and two fp64 FMAs: 3.5 to 5 instructions of 4 cycles for 64
 // elements, and about 100 more a round for the sums.  Measured, HVP in TB/s of stored bytes: E4M3 N = 4 10^6, D = 100 4.6;
 // N = 10^5, D = 8192 4.6, D = 20 000 4.4 (474 us); E2M1 3.1, 2.8, 2.7 (391 us); A v 5.9 and 4.2 at most.
+// (One wave a round for the gradient's coefficients, handed on through LDS and a second barrier: 5 to 12 % longer.)
 #include "vt_mx.h"
 #include <type_traits>
 #include <utility>
