@@ -12,8 +12,6 @@ blocks of 32 columns, one scale byte (a power of two) and 32 codes each: 33 or 1
 
 The reference keeps its arrays in fp64 and has no counterpart.
 """
-import contextlib
-
 import torch
 
 from . import _lib, device as dev
@@ -30,16 +28,6 @@ def check_format(format):
     return format
 
 
-_here = contextlib.nullcontext()
-
-
-def on_device(device):
-    """Context in which ``device`` is the current one (a kernel is launched on the current device)."""
-    if device.index == torch.cuda.current_device():
-        return _here
-    return torch.cuda.device(device)
-
-
 # torch.cuda.current_stream(device).cuda_stream without the Stream object (2.8 -> 0.1 us a call)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
@@ -49,6 +37,17 @@ def stream_of(device):
     if _raw_stream is not None:
         return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def call(name, device, run):
+    """``run(stream)``, a call of the entry point ``name``, with ``device`` the current one (kernels are launched there)."""
+    if device.index == torch.cuda.current_device():
+        code = run(stream_of(device))
+    else:
+        with torch.cuda.device(device):
+            code = run(stream_of(device))
+    if code != _lib.VT_OK:
+        _lib.check(code, name)
 
 
 class CompactRows:
@@ -113,10 +112,9 @@ class CompactRows:
             raise TypeError("dequantise: dtype must be one of %s" % (tuple(TYPE),))
         lib = dev.require_gpu()
         device, shape = self.device, self.shape
-        out = torch.empty(shape, dtype=dtype, device=device)
-        with on_device(device):
-            _lib.check(lib.vt_mx_dequantise(self.c_format(), *self.c_args(), *shape, TYPE[dtype], out.data_ptr(),
-                                            self.D, stream_of(device)), "vt_mx_dequantise")
+        out = torch.empty(*shape, dtype=dtype, device=device)
+        call("vt_mx_dequantise", device, lambda stream: lib.vt_mx_dequantise(
+            self.c_format(), *self.c_args(), *shape, TYPE[dtype], out.data_ptr(), self.D, stream))
         return out
 
     def __repr__(self):
@@ -133,7 +131,8 @@ def quantise(X, format="mxfp8", device=None):
     if isinstance(X, torch.Tensor):
         if X.dtype not in TYPE:
             raise TypeError("quantise: X must be float64, float32, bfloat16 or float16, got %s" % X.dtype)
-        X = X.detach()
+        if X.requires_grad:
+            X = X.detach()
         if device is not None or not X.is_cuda:
             X = dev.to_device(X, device, dtype=X.dtype)
     else:
@@ -145,9 +144,8 @@ def quantise(X, format="mxfp8", device=None):
         X = X.contiguous()
     nb = (D + BLOCK - 1) // BLOCK
     width, at = nb * _BLOCK_BYTES[format], X.device
-    codes = torch.empty((N, width), dtype=torch.uint8, device=at)
-    scales = torch.empty((N, nb), dtype=torch.uint8, device=at)
-    with on_device(at):
-        _lib.check(lib.vt_mx_quantise(TYPE[X.dtype], X.data_ptr(), dev.ld(X), N, D, _lib.MX_FORMAT[format],
-                                      codes.data_ptr(), width, scales.data_ptr(), nb, stream_of(at)), "vt_mx_quantise")
+    codes = torch.empty(N, width, dtype=torch.uint8, device=at)      # (sizes one by one: 0.4 us less than as a tuple)
+    scales = torch.empty(N, nb, dtype=torch.uint8, device=at)
+    call("vt_mx_quantise", at, lambda stream: lib.vt_mx_quantise(
+        TYPE[X.dtype], X.data_ptr(), dev.ld(X), N, D, _lib.MX_FORMAT[format], codes.data_ptr(), width, scales.data_ptr(), nb, stream))
     return CompactRows._made(codes, scales, D, format)

@@ -2,7 +2,7 @@
 import torch
 
 from . import _lib, device as dev
-from .compact import CompactRows, TYPE as _MX_TYPE, on_device, stream_of
+from .compact import CompactRows, TYPE as _MX_TYPE, call
 
 _ws_cache = {}
 
@@ -61,10 +61,13 @@ def _compact(name, X, lead, tail):
     belongs to the call (and, under capture, to the graph): two graphs never share one."""
     lib = dev.require_gpu()
     device = X.device
-    with on_device(device):
+
+    def run(stream):
         nbytes = lib.vt_mx_rows_workspace_bytes(*X.shape)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        _lib.check(getattr(lib, name)(*lead, X.c_format(), *X.c_args(), *tail, ws.data_ptr(), nbytes, stream_of(device)), name)
+        return getattr(lib, name)(*lead, X.c_format(), *X.c_args(), *tail, ws.data_ptr(), nbytes, stream)
+
+    call(name, device, run)
 
 
 def _compact_glm(name, obj, theta, w, outs, prior=()):
@@ -244,7 +247,7 @@ def gemm_tn(A, B, rowscale=None, alpha=1.0, bias=None, out=None):
 def _matrix_out(out, shape, dtypes, device):
     """``out`` of a float product, checked, or a new tensor of the first type."""
     if out is None:
-        return torch.empty(shape, dtype=dtypes[0], device=device)
+        return torch.empty(*shape, dtype=dtypes[0], device=device)
     if out.shape != shape or out.dtype not in dtypes or out.device != device or (out.numel() and (
             out.stride(1) != 1 and out.shape[1] > 1 or dev.ld(out) < shape[1])):
         raise ValueError("out must be a %s row-major tensor of %s on %s" % (shape, " or ".join(map(str, dtypes)), device))
@@ -272,12 +275,15 @@ def _compact_gemm_tn(A, B, rowscale, alpha, bias, out):
     rowscale = None if rowscale is None else _vector(rowscale, N, A, "rowscale")
     bias = _bias(bias, Db, A.device)
     out = _matrix_out(out, (Da, Db), (torch.float32,), A.device)
-    with on_device(A.device):
+
+    def run(stream):
         nbytes = lib.vt_mx_gemm_tn_workspace_bytes(N, Da, Db)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=A.device)
-        _lib.check(lib.vt_mx_gemm_tn(A.c_format(), *A.c_args(), Da, _MX_TYPE[B.dtype], B.data_ptr(), dev.ld(B), Db,
-                                     dev.ptr(rowscale), N, float(alpha), dev.ptr(bias), out.data_ptr(), dev.ld(out),
-                                     ws.data_ptr(), nbytes, stream_of(A.device)), "vt_mx_gemm_tn")
+        return lib.vt_mx_gemm_tn(A.c_format(), *A.c_args(), Da, _MX_TYPE[B.dtype], B.data_ptr(), dev.ld(B), Db,
+                                 dev.ptr(rowscale), N, float(alpha), dev.ptr(bias), out.data_ptr(), dev.ld(out),
+                                 ws.data_ptr(), nbytes, stream)
+
+    call("vt_mx_gemm_tn", A.device, run)
     return out
 
 
@@ -292,12 +298,14 @@ def gemm_nt(A, B, alpha=1.0, bias=None, out=None):
     M, N = A.shape[0], B.shape[0]
     bias = _bias(bias, N, A.device)
     out = _matrix_out(out, (M, N), (torch.float32, torch.bfloat16), A.device)
-    with on_device(A.device):
+
+    def run(stream):
         nbytes = lib.vt_mx_gemm_nt_workspace_bytes(M, N, A.D)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=A.device) if nbytes else None
-        _lib.check(lib.vt_mx_gemm_nt(*A.c_args(), M, *B.c_args(), N, A.D, float(alpha), dev.ptr(bias),
-                                     _MX_TYPE[out.dtype], out.data_ptr(), dev.ld(out), dev.ptr(ws), nbytes,
-                                     stream_of(A.device)), "vt_mx_gemm_nt")
+        return lib.vt_mx_gemm_nt(*A.c_args(), M, *B.c_args(), N, A.D, float(alpha), dev.ptr(bias), _MX_TYPE[out.dtype],
+                                 out.data_ptr(), dev.ld(out), dev.ptr(ws), nbytes, stream)
+
+    call("vt_mx_gemm_nt", A.device, run)
     return out
 
 
