@@ -101,7 +101,10 @@ class CompactRows:
 
     def c_args(self):
         """codes, ldc, scales, lds of the C-ABI."""
-        return self.codes.data_ptr(), dev.ld(self.codes), self.scales.data_ptr(), dev.ld(self.scales)
+        codes, scales = self.codes, self.scales
+        if codes.shape[0] > 1:
+            return codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(0)
+        return codes.data_ptr(), codes.shape[1], scales.data_ptr(), scales.shape[1]
 
     def c_format(self):
         return _lib.MX_FORMAT[self.format]
