@@ -104,3 +104,23 @@ def test_objective_and_panels_take_compact_rows_as_they_are():
             va.WeightedGLMObjective(X, y, family="gaussian", device=device)
     g = torch.randn((50, 9), device="cuda")
     assert torch.equal(rows.gemm_tn_tiled(X, g, tile=32), rows.gemm_tn(X, g))
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("n,da,db,start", [(1000, 64, 33, 1), (1000, 64, 33, 0), (127, 40, 301, 1), (1, 40, 5, 3), (9000, 300, 129, 1)])
+def test_gemm_tn_rows_that_share_a_word(kind, n, da, db, start):
+    """Odd rows without a gap: what lies before the first row, behind the last one and in the next slab's first row shares
+    a word with a row that is read, and must not reach the result, not as 0 * inf either."""
+    torch = _torch()
+    from vittles_amd import compact, rows
+    X = compact.quantise(torch.ones((n, da), device="cuda"), "mxfp8")
+    flat = torch.full((n * db + 8,), float("nan"), dtype=getattr(torch, kind), device="cuda")
+    g = flat[start:start + n * db].view(n, db)
+    g.fill_(1.0)
+    for scale in (None, torch.ones(n, dtype=torch.float64, device="cuda")):
+        g.fill_(1.0)
+        assert torch.equal(rows.gemm_tn(X, g, rowscale=scale), torch.full((da, db), float(n), device="cuda"))
+        g[::64, 0] = float("inf")           # the first rows of all slabs among them
+        want = torch.full((da, db), float(n), device="cuda")
+        want[:, 0] = float("inf")
+        assert torch.equal(rows.gemm_tn(X, g, rowscale=scale), want)

@@ -12,7 +12,7 @@
 // took the same time within 2 %; eight rows of a column side by side in LDS, read with ds_read_b128 at twice the rate of
 // the transposing read (133 against 72 bytes a cycle) and put there by v_perm, 3 to 8 % longer; one chunk ahead instead of
 // two 8 to 18 % longer.  Where the slabs' sums are large, their way out and back counts too (16384 x 4096 x 1000: 15 of
-// 155 us).
+// 155 us).  Odd rows of B cost 0 (float) to 25 % (bfloat16, 16384 x 4096 x 1001: 177 us).
 #include "vt_mx.h"
 #include <type_traits>
 
@@ -90,6 +90,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tn(MxTN a, int tiles_d, 
     const int d0 = tile / tiles_k * S::BM, k0 = tile % tiles_k * S::BN;
     const int width = mx_blocks(a.Da) * kMxBlock;
 
+    // VEC: B's rows begin on 4 bytes (B's last column may bring the 2 bytes behind it, never another 4).  Else, in 16-bit
+    // types: the aligned words around a piece, shifted into place when it goes to LDS (a row's parity is the same in every
+    // chunk).
+    const unsigned odd_base = VEC ? 0 : (unsigned)(uintptr_t)a.B & 2;
     unsigned va[S::kLoadsA], vs[S::kLoadsA], vb[S::kLoadsB];
 #pragma unroll
     for (int i = 0; i < S::kLoadsA; ++i) {
@@ -101,12 +105,13 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tn(MxTN a, int tiles_d, 
 #pragma unroll
     for (int i = 0; i < S::kLoadsB; ++i) {
         const int e = tid + S::kThreads * i, c = k0 + e % (S::BN / 8) * 8;
-        vb[i] = c < a.Db ? (e / (S::BN / 8) * (unsigned)a.ldb + c) * (unsigned)sizeof(T) : kNowhere;
+        vb[i] = c < a.Db ? odd_base + (e / (S::BN / 8) * (unsigned)a.ldb + c) * (unsigned)sizeof(T) : kNowhere;
     }
     struct Chunk {
         W ca[S::kLoadsA];
         unsigned sc[S::kLoadsA];
         u32x4 cb[S::kLoadsB][sizeof(T) / 2];
+        unsigned tail[VEC ? 1 : S::kLoadsB];
         double rs[SCALED ? S::kLoadsB : 1];
     };
     // rows behind the slab's end come as 0; columns of a piece behind the last one are the next row's and end in columns
@@ -115,9 +120,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tn(MxTN a, int tiles_d, 
         const int64_t left = n_hi - n0;
         const auto ra = mx_rsrc(a.codes + n0 * a.ldc, left > 0 ? (left - 1) * a.ldc + (FMT == VT_MX_FP8 ? width : width / 2) : 0);
         const auto rs = mx_rsrc(a.scales + n0 * a.lds, left > 0 ? (left - 1) * a.lds + width / kMxBlock : 0);
-        constexpr int kWide = 16 / sizeof(T);        // a load that holds a row's last column ends inside its 16 bytes
-        const int64_t last = (a.Db + kWide - 1) / kWide * kWide;
-        const auto rb = mx_rsrc((const T*)a.B + n0 * a.ldb, left > 0 ? ((left - 1) * a.ldb + last) * (int64_t)sizeof(T) : 0);
+        const auto rb = mx_rsrc((const uint8_t*)a.B - odd_base + n0 * a.ldb * (int64_t)sizeof(T),
+                                left > 0 ? (odd_base + ((left - 1) * a.ldb + a.Db) * (int64_t)sizeof(T) + 3) / 4 * 4 : 0);
 #pragma unroll
         for (int i = 0; i < S::kLoadsA; ++i) {
             if constexpr (FMT == VT_MX_FP8) x.ca[i] = __builtin_bit_cast(W, __builtin_amdgcn_raw_buffer_load_b128(ra, va[i], 0, 0));
@@ -131,22 +135,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tn(MxTN a, int tiles_d, 
                 for (int j = 0; j < (int)sizeof(T) / 2; ++j)
                     x.cb[i][j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rb, vb[i] + 16 * j, 0, 0));
             } else {
-                // rows at any alignment: wide loads at the element's own, single ones at the row's end
-                typedef typename Unaligned16<sizeof(T)>::type wide;
-                const int e = tid + S::kThreads * i, c = k0 + e % (S::BN / 8) * 8;
-                const int64_t n = n0 + e / (S::BN / 8);
-                const T* p = (const T*)a.B + n * a.ldb + c;
-#pragma unroll
-                for (int j = 0; j < (int)sizeof(T) / 2; ++j) x.cb[i][j] = u32x4{0, 0, 0, 0};
-                if (n < n_hi && c + 8 <= a.Db) {
-#pragma unroll
-                    for (int j = 0; j < (int)sizeof(T) / 2; ++j) x.cb[i][j] = ((const wide*)p)[j];
-                } else if (n < n_hi && c < a.Db) {
-                    T v[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[j] = c + j < a.Db ? p[j] : (T)0.0f;
-                    __builtin_memcpy(x.cb[i], v, sizeof(v));
-                }
+                // (a row behind the last one shares a word with it)
+                const unsigned off = (tid + S::kThreads * i) / (S::BN / 8) < left ? vb[i] & ~3u : kNowhere;
+                x.cb[i][0] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rb, off, 0, 0));
+                x.tail[i] = __builtin_amdgcn_raw_buffer_load_b32(rb, off + 16, 0, 0);
             }
             if constexpr (SCALED) {
                 const int64_t n = n0 + (tid + S::kThreads * i) / (S::BN / 8);
@@ -183,11 +175,18 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tn(MxTN a, int tiles_d, 
         for (int i = 0; i < S::kLoadsB; ++i) {
             const int e = tid + S::kThreads * i;
             uint8_t* p = base + S::kA + e / (S::BN / 8) * S::kPitchB + e % (S::BN / 8) * 16;
+            u32x4 b8[sizeof(T) / 2];
+            __builtin_memcpy(b8, x.cb[i], sizeof(b8));
+            if constexpr (!VEC) {
+                const unsigned by = (vb[i] & 2) * 8;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) b8[0][j] = __builtin_amdgcn_alignbit(j < 3 ? b8[0][j + 1] : x.tail[i], b8[0][j], by);
+            }
             if constexpr (PARTS == 1) {
-                *(u32x4*)p = x.cb[i][0];
+                *(u32x4*)p = b8[0];
             } else {
                 T c[8];
-                __builtin_memcpy(c, x.cb[i], sizeof(c));
+                __builtin_memcpy(c, b8, sizeof(c));
                 u32x4 w[PARTS];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -351,12 +350,18 @@ int launch(const MxTN& a, const TnPlan& p, hipStream_t st) {
     return vt_launch_status();
 }
 
+template <int FMT, typename T, bool SCALED, bool VEC>
+int launch(const MxTN& a, const TnPlan& p, hipStream_t st) {
+    if (p.bn == 256) return launch<FMT, T, SCALED, 4, 2, 2, 4, VEC>(a, p, st);
+    if (p.bm == 256) return launch<FMT, T, SCALED, 4, 2, 2, 2, VEC>(a, p, st);
+    return launch<FMT, T, SCALED, 2, 1, 2, 2, VEC>(a, p, st);
+}
+
 template <int FMT, typename T, bool SCALED>
 int launch(const MxTN& a, const TnPlan& p, hipStream_t st) {
-    const bool vec = (uintptr_t)a.B % 16 == 0 && a.ldb * (int64_t)sizeof(T) % 16 == 0;
-    if (p.bn == 256) return vec ? launch<FMT, T, SCALED, 4, 2, 2, 4, true>(a, p, st) : launch<FMT, T, SCALED, 4, 2, 2, 4, false>(a, p, st);
-    if (p.bm == 256) return vec ? launch<FMT, T, SCALED, 4, 2, 2, 2, true>(a, p, st) : launch<FMT, T, SCALED, 4, 2, 2, 2, false>(a, p, st);
-    return vec ? launch<FMT, T, SCALED, 2, 1, 2, 2, true>(a, p, st) : launch<FMT, T, SCALED, 2, 1, 2, 2, false>(a, p, st);
+    if constexpr (sizeof(T) == 2)
+        if ((uintptr_t)a.B % 4 != 0 || a.ldb % 2 != 0) return launch<FMT, T, SCALED, false>(a, p, st);
+    return launch<FMT, T, SCALED, true>(a, p, st);
 }
 
 template <int FMT, typename T>
@@ -381,6 +386,7 @@ extern "C" int vt_mx_gemm_tn(int format, const void* codes, int64_t ldc, const v
                              const float* bias, float* C, int64_t ldo, void* ws, size_t ws_bytes, void* stream) {
     if (!mx_rows_ok(format, codes, ldc, scales, lds, N, Da) || Db < 1 || !C || ldo < Db) return VT_ERR_BAD_ARG;
     if (type < VT_TYPE_F32 || type > VT_TYPE_F16 || (N > 0 && (!B || ldb < Db))) return VT_ERR_BAD_ARG;
+    if ((uintptr_t)B % (type == VT_TYPE_F32 ? 4 : 2)) return VT_ERR_BAD_ARG;
     const TnPlan p = plan(N, Da, Db);
     if (!ws || ws_bytes < vt_mx_gemm_tn_workspace_bytes(N, Da, Db)) return VT_ERR_WORKSPACE;
     if (N <= 1) ldb = (Db + 7) / 8 * 8;      // a single row has no stride
