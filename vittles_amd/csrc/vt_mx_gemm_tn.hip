@@ -11,8 +11,9 @@
 // way to LDS).  Reading operands a step ahead, spreading the writes to LDS over the steps, or fixing the order of the two
 // took the same time within 2 %; eight rows of a column side by side in LDS, read with ds_read_b128 at twice the rate of
 // the transposing read (133 against 72 bytes a cycle) and put there by v_perm, 3 to 8 % longer; one chunk ahead instead of
-// two 8 to 18 % longer.  Where the slabs' sums are large, their way out and back counts too (16384 x 4096 x 1000: 15 of
-// 155 us).  Odd rows of B cost 0 (float) to 25 % (bfloat16, 16384 x 4096 x 1001: 177 us).
+// two 8 to 18 % longer.  What is left is power: 16384 x 4096 x 1000 takes 140 to 150 us, 15 of them the
+// slabs' way out and back, and 121 if B is zeros.  Odd rows of B cost 0 (float) to 25 % (bfloat16, 16384 x 4096 x 1001:
+// 177 us).
 #include "vt_mx.h"
 #include <type_traits>
 
