@@ -1,0 +1,45 @@
+"""GPU tests of compact rows at the largest sizes: more rows or columns than the threads of one launch."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def _torch():
+    import torch
+    assert torch.cuda.is_available(), "GPU tests need a HIP device"
+    return torch
+
+
+@pytest.mark.parametrize("side", ["rows of A", "rows of B"])
+def test_gemm_nt_more_rows_than_a_launch_holds(side):
+    """2^28 + 21 rows against three: one block of 32 columns each.  The codes stand for whole numbers whose sums stay
+    below 2^24: products are exact in float, and the bfloat16 result is their one rounding."""
+    torch = _torch()
+    from vittles_amd import compact, rows
+    many, few, d = (1 << 28) + 21, 3, 32
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    # an even E2M1 index is 0, 1, 2 or 4: whole numbers in both halves of a byte
+    codes = torch.randint(0, 256, (many, 16), generator=gen, dtype=torch.uint8, device="cuda").bitwise_and_(0xEE)
+    scales = torch.randint(126, 130, (many, 1), generator=gen, dtype=torch.uint8, device="cuda").add_(1)
+    long = compact.CompactRows(codes, scales, d, "mxfp4")
+    short = compact.CompactRows(codes[7:7 + few].clone(), scales[7:7 + few].clone(), d, "mxfp4")
+    short_values = short.dequantise(torch.float64)
+    if side == "rows of B":
+        bias = (torch.arange(many, device="cuda") % 251).to(torch.float32)
+        out = torch.full((few, many), float("nan"), dtype=torch.bfloat16, device="cuda")
+        rows.gemm_nt(short, long, bias=bias, out=out)
+    else:
+        bias = torch.tensor([1.0, -2.0, 5.0], device="cuda")
+        out = torch.full((many, few), float("nan"), dtype=torch.bfloat16, device="cuda")
+        rows.gemm_nt(long, short, bias=bias, out=out)
+    # the rows around every border of the launches, and a stretch of the others
+    for lo in (0, (1 << 27) - 40, (1 << 28) - 40, 3 << 26, many - 60):
+        part = slice(lo, min(many, lo + 100))
+        x = compact.CompactRows(codes[part], scales[part], d, "mxfp4").dequantise(torch.float64)
+        if side == "rows of B":
+            want, got = short_values @ x.t().contiguous() + bias[part].double(), out[:, part]
+        else:
+            want, got = x @ short_values.t().contiguous() + bias.double(), out[part]
+        assert float(want.abs().max()) < 1 << 24
+        assert torch.equal(got, want.to(torch.bfloat16)), lo
+    assert not bool(torch.isnan(out).any())

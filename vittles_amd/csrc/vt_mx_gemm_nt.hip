@@ -306,15 +306,26 @@ __global__ __launch_bounds__(256) void k_mx_nt_few(MxNT a, MxFew f) {
     }
 }
 
+// A launch holds fewer than 2^32 threads: 2^27 of the many rows are 2^31 of them, more rows go in several launches.
+constexpr int64_t kManyRows = 1 << 27;
+
 template <int MT, typename OutT>
-int launch_few(const MxNT& a, hipStream_t st) {
-    const bool swap = a.N < a.M;
+int launch_few(const MxNT& whole, hipStream_t st) {
+    const bool swap = whole.N < whole.M;
+    MxNT a = whole;
     MxFew f = swap ? MxFew{a.ca, a.sa, a.cb, a.sb, a.ldca, a.ldsa, a.ldcb, a.ldsb, a.M, a.N}
                    : MxFew{a.cb, a.sb, a.ca, a.sa, a.ldcb, a.ldsb, a.ldca, a.ldsa, a.N, a.M};
-    const dim3 grid((unsigned)((f.many + 15) / 16), (unsigned)((f.few + 16 * MT - 1) / (16 * MT)));
-    if (swap) hipLaunchKernelGGL((k_mx_nt_few<MT, true, OutT>), grid, dim3(256), 0, st, a, f);
-    else hipLaunchKernelGGL((k_mx_nt_few<MT, false, OutT>), grid, dim3(256), 0, st, a, f);
-    return vt_launch_status();
+    for (int64_t left = f.many; left > 0; left -= kManyRows) {
+        f.many = std::min(left, kManyRows);
+        const dim3 grid((unsigned)((f.many + 15) / 16), (unsigned)((f.few + 16 * MT - 1) / (16 * MT)));
+        if (swap) hipLaunchKernelGGL((k_mx_nt_few<MT, true, OutT>), grid, dim3(256), 0, st, a, f);
+        else hipLaunchKernelGGL((k_mx_nt_few<MT, false, OutT>), grid, dim3(256), 0, st, a, f);
+        if (int rc = vt_launch_status()) return rc;
+        f.cm += f.many * f.ldcm, f.sm += f.many * f.ldsm;
+        a.C = (OutT*)a.C + f.many * (swap ? a.ldc : 1);
+        if (!swap && a.bias) a.bias += f.many;
+    }
+    return VT_OK;
 }
 
 struct NtPlan {
