@@ -355,7 +355,8 @@ int    vt_mx_dequantise(int format, const void* codes_dev, int64_t ldc, const vo
                         int64_t N, int D, int type, void* out_dev, int64_t ldo, void* stream);
 
 /* Row operators on compact rows: arguments, results and their fp64 vectors and sums as vt_glm_link / _grad / _value /
- * _hvp / vt_gemv / vt_gemv_t2 (u2 may be NULL: vt_gemv_t).  D >= 1 without an upper limit. */
+ * _hvp / vt_gemv / vt_gemv_t2 (u2 may be NULL: vt_gemv_t).  1 <= D <= 2^30 (past 20352 in two passes over
+ * the rows). */
 size_t vt_mx_rows_workspace_bytes(int64_t N, int D);
 int    vt_mx_glm_link(int family, int format, const void* codes_dev, int64_t ldc, const void* scales_dev, int64_t lds,
                       const double* theta_dev, const double* y_dev, const double* w_dev, const double* offset_dev,

@@ -43,3 +43,25 @@ def test_gemm_nt_more_rows_than_a_launch_holds(side):
         assert float(want.abs().max()) < 1 << 24
         assert torch.equal(got, want.to(torch.bfloat16)), lo
     assert not bool(torch.isnan(out).any())
+
+
+def test_row_operators_more_columns_than_a_launch_holds():
+    """Two rows of 2^27 + 37 columns: whole numbers, exact sums."""
+    torch = _torch()
+    from vittles_amd import compact, rows
+    n, d = 2, (1 << 27) + 37
+    nb = (d + 31) // 32
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    codes = torch.randint(0, 256, (n, nb * 16), generator=gen, dtype=torch.uint8, device="cuda").bitwise_and_(0xEE)
+    codes[:, (d - 1) // 2 + 1:] = 0                       # the columns behind the last one
+    codes[:, (d - 1) // 2] &= 0x0F
+    scales = torch.randint(127, 131, (n, nb), generator=gen, dtype=torch.uint8, device="cuda")
+    X = compact.CompactRows(codes, scales, d, "mxfp4")
+    x = X.dequantise(torch.float64)
+    u = torch.tensor([3.0, -2.0], dtype=torch.float64, device="cuda")
+    assert torch.equal(rows.gemv_t(X, u), 3.0 * x[0] - 2.0 * x[1])
+    v = torch.randint(-2, 3, (d,), generator=gen, device="cuda").to(torch.float64)
+    z = torch.stack([(x[0] * v).sum(), (x[1] * v).sum()])
+    assert torch.equal(rows.gemv(X, v), z)
+    prior = torch.randint(1, 4, (d,), generator=gen, device="cuda").to(torch.float64)
+    assert torch.equal(rows.glm_hvp(X, u, v, prior=prior), x[0] * (3.0 * z[0]) + x[1] * (-2.0 * z[1]) + prior * v)

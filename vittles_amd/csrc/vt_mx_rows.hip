@@ -512,12 +512,13 @@ __global__ __launch_bounds__(256) void k_mx_columns(MxRows a) {
         if (g * 8 + i < a.D) out[g * 8 + i] = acc[i];
 }
 
-// out[c] = sum_p part[p][c] + beta[c] bvec[c], 32 columns a workgroup, 32 groups each summing every 32nd slab.
-__global__ __launch_bounds__(1024) void k_mx_finalize(const double* part, int P, int D, const double* beta, const double* bvec,
-                                                      double beta_scalar, double* out) {
+// out[c] = sum_p part[p][c] + beta[c] bvec[c] from column c0 on, 32 columns a workgroup, 32 groups each summing every 32nd
+// slab.
+__global__ __launch_bounds__(1024) void k_mx_finalize(const double* part, int P, int D, int c0, const double* beta,
+                                                      const double* bvec, double beta_scalar, double* out) {
     __shared__ double sh[32][33];
     const int cl = threadIdx.x & 31, grp = threadIdx.x >> 5;
-    const int c = blockIdx.x * 32 + cl;
+    const int c = c0 + blockIdx.x * 32 + cl;
     double s = 0.0;
     if (c < D)
         for (int p = grp; p < P; p += 32) s += part[(int64_t)p * D + c];
@@ -647,7 +648,11 @@ int run(int format, const MxRows& a, const RowsPlan& p, hipStream_t st) {
 
 int finalize(const double* part, int P, int D, const double* beta, const double* bvec, double beta_scalar, double* out,
              hipStream_t st) {
-    hipLaunchKernelGGL(k_mx_finalize, dim3((D + 31) / 32), dim3(1024), 0, st, part, P, D, beta, bvec, beta_scalar, out);
+    // (a launch holds fewer than 2^32 threads: 2^26 columns are 2^31 of them)
+    constexpr int kPanel = 1 << 26;
+    for (int c0 = 0; c0 < D; c0 += kPanel)
+        hipLaunchKernelGGL(k_mx_finalize, dim3((std::min(D - c0, kPanel) + 31) / 32), dim3(1024), 0, st, part, P, D, c0, beta, bvec,
+                           beta_scalar, out);
     return vt_launch_status();
 }
 
