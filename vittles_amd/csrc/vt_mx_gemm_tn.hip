@@ -379,7 +379,9 @@ int launch(int type, const MxTN& a, const TnPlan& p, hipStream_t st) {
 
 extern "C" size_t vt_mx_gemm_tn_workspace_bytes(int64_t N, int Da, int Db) {
     if (N < 0 || Da < 1 || Db < 1) return 0;
-    return (size_t)plan(N, Da, Db).slabs * Da * Db * sizeof(float);
+    // one slab goes straight to C; a float all the same, so that what a caller allocates has an address
+    const int slabs = plan(N, Da, Db).slabs;
+    return slabs > 1 ? (size_t)slabs * Da * Db * sizeof(float) : sizeof(float);
 }
 
 extern "C" int vt_mx_gemm_tn(int format, const void* codes, int64_t ldc, const void* scales, int64_t lds, int Da, int type,
