@@ -387,7 +387,10 @@ int    vt_mx_gemm_nt(const void* codes_a_dev, int64_t ldca, const void* scales_a
                      size_t ws_bytes, void* stream);
 /* C (Da, Db) = alpha * A^T diag(rowscale) B + 1 bias^T for compact rows A (N, Da) and B (N, Db) of type F32, BF16 or
  * F16: the gradient of a linear layer's weights from its stored activations.  The product rowscale * B is rounded once
- * to float; products are exact, sums and C are float; rowscale (N,) double or NULL, bias (Db,) float or NULL. */
+ * to float; products are exact, sums and C are float; rowscale (N,) double or NULL, bias (Db,) float or NULL.  Numbers end
+ * at 2^-133: a value of A is taken to the nearest multiple of it, what a float of B (or rowscale * B) has below it is cut
+ * off.  Both are exact for values of A in blocks whose largest magnitude is 2^-116 and up (E2M1: all) and floats of 2^-110
+ * and up. */
 size_t vt_mx_gemm_tn_workspace_bytes(int64_t N, int Da, int Db);
 int    vt_mx_gemm_tn(int format, const void* codes_dev, int64_t ldc, const void* scales_dev, int64_t lds, int Da,
                      int type, const void* B_dev, int64_t ldb, int Db, const double* rowscale_dev, int64_t N,

@@ -143,3 +143,34 @@ def test_gemm_tn_whole_numbers(n, da, db, kernel, split, kind, bits, weighted):
     rows.gemm_tn(X, B, rowscale=w if weighted else None, alpha=-2.0, bias=bias, out=buf[:da, 1:db + 1])
     assert torch.equal(buf[:da, 1:db + 1], (-2.0 * ref + bias.double()).float())
     assert bool((buf[da] == 7).all() and (buf[:, 0] == 7).all() and (buf[:, db + 1:] == 7).all())
+
+
+def test_gemm_tn_smallest_numbers():
+    """A is taken to the nearest multiple of 2^-133 (ties to even), a float of B cut to one; larger numbers are exact."""
+    torch = _torch()
+    from vittles_amd import compact, rows
+    step = 2.0 ** -133
+    for fmt, width in (("mxfp8", 256), ("mxfp4", 128)):
+        # a row for each scale byte 0 .. 7, all bytes as codes but the NaN of E4M3
+        codes = (torch.arange(width, device="cuda") * (256 // width) + (fmt == "mxfp4")).to(torch.uint8).expand(8, width).clone()
+        if fmt == "mxfp8":
+            codes[:, [0x7F, 0xFF]] = 0x7E
+        d = width * (1 if fmt == "mxfp8" else 2)
+        scales = torch.arange(8, dtype=torch.uint8, device="cuda")[:, None].expand(8, d // 32).clone()
+        X = compact.CompactRows(codes, scales, d, fmt)
+        x = X.dequantise(torch.float64)
+        near = torch.round(x / step) * step
+        assert torch.equal(near[3:], x[3:]) and (fmt == "mxfp8") != torch.equal(near[:3], x[:3])
+        for kind in (torch.bfloat16, torch.float32):
+            g = (2.0 ** 100 * torch.eye(8, device="cuda")).to(kind)
+            for w in (None, torch.ones(8, dtype=torch.float64, device="cuda")):
+                assert torch.equal(rows.gemm_tn(X, g, rowscale=w).double(), near.t() * 2.0 ** 100)
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    X = compact.quantise(torch.full((1, 40), 2.0 ** 20, device="cuda"), "mxfp8")
+    b = (1.0 + torch.rand(900, generator=gen, device="cuda")) * torch.sign(torch.randn(900, generator=gen, device="cuda"))
+    b = torch.ldexp(b.double(), torch.arange(900, device="cuda") % 50 - 149).float()[None, :]
+    cut = torch.trunc(b.double() / step) * step
+    large = b.abs() >= 2.0 ** -110
+    assert torch.equal(cut[large], b.double()[large]) and bool(large.any())
+    for w in (None, torch.ones(1, dtype=torch.float64, device="cuda")):
+        assert torch.equal(rows.gemm_tn(X, b, rowscale=w).double(), (cut * 2.0 ** 20).expand(40, 900))

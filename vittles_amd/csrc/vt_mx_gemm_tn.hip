@@ -1,8 +1,10 @@
 // Gradient of a linear layer's weights from stored activations: C (Da, Db) = alpha A^T diag(rowscale) B + 1 bias^T with
 // compact rows A (N, Da) and float, bfloat16 or half rows B (N, Db), on v_mfma_f32_32x32x16_bf16.
-// A code times its scale IS a bfloat16 (4 significant bits at most; v_cvt_scalef32_pk_bf16_fp8 / _fp4), so A enters the
-// product exactly.  B is cut into bfloat16 parts that add up to it: one for bfloat16, two for half (11 bits), three for
-// float (24 bits) and for anything times rowscale (rounded once to float).  Every product is exact; sums are float.
+// A code times its scale has 4 significant bits at most and is a bfloat16 (v_cvt_scalef32_pk_bf16_fp8 / _fp4) down to that
+// type's smallest step, 2^-133: A enters the product exactly, but for the finest codes of E4M3 blocks with scale bytes 0 to
+// 2 (largest magnitude below 2^-116), which are rounded to that step.  B is cut into bfloat16 parts that add up to it: one
+// for bfloat16, two for half (11 bits), three for float (24 bits) and for anything times rowscale (rounded once to float);
+// the parts of a float below 2^-110 end at 2^-133 too, what is finer is cut off.  Products are exact; sums are float.
 // Both operands are contracted along the rows, across which they lie in memory: a chunk of rows is staged as it lies and
 // read with the transposing LDS read (ds_read_b64_tr_b16), 4 rows x 16 columns a quarter wave.
 // The long axis N is cut into slabs; a slab's sums are float and the slabs are added in a fixed order.

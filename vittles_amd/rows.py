@@ -213,7 +213,8 @@ def gemm_tn(A, B, rowscale=None, alpha=1.0, bias=None, out=None):
 
     ``A`` as ``CompactRows``: the gradient of a linear layer's weights from its stored activations.  ``B`` (the gradient
     of the layer's outputs) is float32, bfloat16 or float16, ``rowscale`` float64, ``bias`` float32; products are exact,
-    sums and ``out`` float32."""
+    sums and ``out`` float32.  (Values of A are taken to the nearest multiple of 2^-133 and float32 numbers of B cut to
+    one: exact but in blocks of A below 2^-116 and for numbers of B below 2^-110.)"""
     if isinstance(A, CompactRows):
         return _compact_gemm_tn(A, B, rowscale, alpha, bias, out)
     lib = dev.require_gpu()
