@@ -331,8 +331,8 @@ int    vt_gemm_tn_f32b(const double* A_dev, int64_t lda, int Da, const float* B_
  * A row of D numbers is cut into nb = ceil(D / 32) blocks of 32 columns.  A block is one scale byte s, standing for
  * 2^(s - 127) (255: the whole block is NaN), and 32 codes: VT_MX_FP8 = E4M3 (1 sign, 4 exponent, 3 mantissa bits; 32
  * bytes a block), VT_MX_FP4 = E2M1 (magnitudes 0 .5 1 1.5 2 3 4 6; 16 bytes a block, the even column in the low half
- * of a byte).  The value of an element is code * 2^(s - 127), in the range of float.  Codes of the columns >= D of the
- * last block are 0.
+ * of a byte).  The value of an element is code * 2^(s - 127) as a float: from 2^128 on an infinity.  Codes of the columns
+ * >= D of the last block are 0.
  *   codes  : (N, ldc) bytes, 16-byte aligned, ldc a multiple of 16, >= nb * 32 (FP8) or nb * 16 (FP4)
  *   scales : (N, lds) bytes, lds >= nb
  * The reference keeps its arrays in fp64 and has no counterpart; the row operators below take the place of the same
@@ -347,7 +347,8 @@ int    vt_gemm_tn_f32b(const double* A_dev, int64_t lda, int Da, const float* B_
 /* codes, scales <- X (N, D; element stride 1, row stride ldx).  Scale: the smallest power of two in 2^-127 .. 2^127
  * with which the largest magnitude of the block still rounds to a finite code, so nothing saturates; codes: round to
  * nearest, ties to even, from the full precision of X.  A block that holds NaN, an infinity or a magnitude that
- * rounds past the largest float gets s = 255 and codes 0. */
+ * rounds past the largest float gets s = 255 and codes 0.  (A float whose code stands for 2^128 is stored and reads as
+ * an infinity: magnitudes from 1.9375 2^127 on in FP8, from 1.75 2^127 on in FP4.) */
 int    vt_mx_quantise(int type, const void* X_dev, int64_t ldx, int64_t N, int D, int format, void* codes_dev,
                       int64_t ldc, void* scales_dev, int64_t lds, void* stream);
 /* out (N, D; row stride ldo) <- the values, rounded to `type` (exact for F32, F64; BF16 too but for subnormals). */

@@ -65,3 +65,21 @@ def test_row_operators_more_columns_than_a_launch_holds():
     assert torch.equal(rows.gemv(X, v), z)
     prior = torch.randint(1, 4, (d,), generator=gen, device="cuda").to(torch.float64)
     assert torch.equal(rows.glm_hvp(X, u, v, prior=prior), x[0] * (3.0 * z[0]) + x[1] * (-2.0 * z[1]) + prior * v)
+
+
+@pytest.mark.parametrize("fmt,border,below", [("mxfp8", 1.9375, 1.875), ("mxfp4", 1.75, 1.5)])
+def test_numbers_that_round_to_the_first_power_past_float(fmt, border, below):
+    """The largest numbers of float: those below the border keep a value, the others have a code that stands for 2^128 and
+    read as infinities of their sign; the rest of the block is as it was."""
+    import numpy as np
+    torch = _torch()
+    from vittles_amd import compact, rows
+    p = 2.0 ** 127
+    last = float(np.nextafter(np.float32(border * p), np.float32(0)))
+    x = torch.tensor([[last, -last, 2.0 ** 125], [border * p, -border * p, 2.0 ** 125]], dtype=torch.float64, device="cuda")
+    inf = float("inf")
+    want = torch.tensor([[below * p, -below * p, 2.0 ** 125], [inf, -inf, 2.0 ** 125]], dtype=torch.float64, device="cuda")
+    for dtype in (torch.float64, torch.float32):
+        X = compact.quantise(x.to(dtype), fmt)
+        assert torch.equal(X.dequantise(torch.float64), want) and torch.equal(X.dequantise(), want.float())
+        assert torch.equal(rows.gemv(X, torch.tensor([1.0, 0.0, 0.0], dtype=torch.float64, device="cuda"))[:1], want[:1, 0])

@@ -4,11 +4,15 @@ What a design matrix is in practice -- the activations that a network hands to i
 digits than fp64 or fp32, and the row operators of this package are bound by its bytes.  ``CompactRows`` keeps a row in
 blocks of 32 columns, one scale byte (a power of two) and 32 codes each: 33 or 17 bytes where fp64 takes 256.
 
-    X8   = compact.quantise(X)                       # E4M3, each element off by at most 2^-4 of its size
+    X8   = compact.quantise(X)                       # E4M3
     obj  = WeightedGLMObjective(X8, y, prior=1.0)    # value, gradient, HVP and the CG route read the 8-bit rows
     hvp  = cg.GLMHessianVectorProduct(obj, theta, w)
     dW   = rows.gemm_tn(X8, dZ)                      # weight gradient of a layer with several outputs
     T    = rows.gemm_nt(compact.quantise(Q, "mxfp4"), compact.quantise(X, "mxfp4"))      # scores of all pairs
+
+An element is off by at most 2^-4 (E4M3) or 2^-2 (E2M1) of its size, or half the smallest step of its block, whichever is
+larger: a number far below the largest of its 32 reads as 0.  The smallest step is at most 2^-16 (E4M3) or 1/7 (E2M1) of the
+block's largest magnitude, but never under 2^-136 (E4M3) or 2^-128 (E2M1).
 
 The reference keeps its arrays in fp64 and has no counterpart.
 """
@@ -128,7 +132,8 @@ def quantise(X, format="mxfp8", device=None):
     """``X`` (N, D) -- numpy, or a float64 / float32 / bfloat16 / float16 tensor -- as ``CompactRows``.
 
     A block's scale is the smallest power of two with which its largest magnitude still rounds to a code; codes are
-    rounded to nearest, ties to even, once.  A block with a NaN, an infinity or a magnitude beyond float32 reads as NaN."""
+    rounded to nearest, ties to even, once.  A block with a NaN, an infinity or a magnitude beyond float32 reads as NaN; a
+    number that rounds to 2^128 (1.9375 2^127 and up in mxfp8, 1.75 2^127 and up in mxfp4) reads as an infinity."""
     check_format(format)
     lib = dev.require_gpu()
     if isinstance(X, torch.Tensor):
