@@ -39,10 +39,10 @@ __device__ __forceinline__ void mx_store(const MxNT& a, int64_t m, int64_t n, fl
 // (LDS-DMA, 16 bytes a lane for codes, 4 for scales) while this one is multiplied.
 // LDS: 16-byte slot j of row r holds block j ^ ((r >> 1) & 7), so the sixteen rows that are read at a time lie in
 // different banks.  The DMA writes slots in lane order; the permutation is in the lanes' addresses.
-// Measured at 8192^3: 296 us = 3.7 PFLOP/s (4096^2 x 8192: 79 us, 3.5).  The codes' way from L2 alone takes 225 (2.1 GB at
-// the ~10 TB/s that two chunks in flight draw), products and operand reads alone 214, writing C 50: the first two overlap,
-// the last does not, a tile's workgroup fills its CU.  Reading operands a step ahead, with the barrier under the last
-// step's products, took the same time.
+// Measured at 8192^3: 295 us from a graph, 315 among other kernels (3.7 and 3.5 PFLOP/s, medians; bfloat16 result 274);
+// 4096^2 x 8192: 79 us, 3.5.  The codes' way from L2 alone takes 225 (2.1 GB at the ~10 TB/s that two chunks in flight
+// draw), products and operand reads alone 214, writing C 50: the first two overlap, the last does not, a tile's workgroup
+// fills its CU.  Reading operands a step ahead, with the barrier under the last step's products, took the same time.
 constexpr int kChunk = 8, kRow = 16 * kChunk, kRowsPerLoad = 1024 / kRow;
 __device__ __forceinline__ int nt_slot(int block, int row) { return 16 * (block ^ ((row >> 1) & 7)); }
 

@@ -8,14 +8,18 @@
 // Both operands are contracted along the rows, across which they lie in memory: a chunk of rows is staged as it lies and
 // read with the transposing LDS read (ds_read_b64_tr_b16), 4 rows x 16 columns a quarter wave.
 // The long axis N is cut into slabs; a slab's sums are float and the slabs are added in a fixed order.
-// Bound: the matrix unit, once a part: 8192 x 4096 x 4096 takes 240 us in bfloat16 (1.15 PFLOP/s; a library product of
-// 8192^3 reaches 1.36), 470 in half, 680 in float and 725 weighted.  Two VALU instructions go with an MFMA (conversion, the
-// way to LDS).  Reading operands a step ahead, spreading the writes to LDS over the steps, or fixing the order of the two
+// What bounds it: 8192 x 4096 x 4096 takes 235 us in bfloat16 (1.17 PFLOP/s; a library product of 8192^3 reaches 1.36), 470
+// in half, 670 in float and 715 weighted.  With one part it is LDS: a chunk of 64 rows costs 48 transposing reads of 512
+// bytes in each of 8 waves, 2730 cycles at 72 bytes a cycle, 512 for the writes and 260 of conflicts, against 2048 of MFMA;
+// measured at 16384 x 4096 x 1000: 4280 cycles a chunk, the matrix unit busy in 48 %.  For 16 rows two parts come to 910
+// cycles of reads and 1024 of MFMA, three to 1138 and 1536.  Two VALU instructions go with an MFMA (conversion, the way to
+// LDS).  Reading operands a step ahead, spreading the writes to LDS over the steps, or fixing the order of the two
 // took the same time within 2 %; eight rows of a column side by side in LDS, read with ds_read_b128 at twice the rate of
 // the transposing read (133 against 72 bytes a cycle) and put there by v_perm, 3 to 8 % longer; one chunk ahead instead of
-// two 8 to 18 % longer.  What is left is power: 16384 x 4096 x 1000 takes 140 to 150 us, 15 of them the
-// slabs' way out and back, and 121 if B is zeros.  Odd rows of B cost 0 (float) to 25 % (bfloat16, 16384 x 4096 x 1001:
-// 177 us).
+// two 8 to 18 % longer.  16384 x 4096 x 1000 takes 140 to 150 us, 15 of them the slabs' way out and back, and 120
+// if B is zeros: the clock that the power leaves (2.0 GHz) has its share.  Odd rows of B cost 0 (float) to 25 % (bfloat16,
+// 16384 x 4096 x 1001: 179 us).  129 to 255 tiles of 256 x 256 go as one slab and leave CUs idle: 16384 x 4096 x 2304, 144
+// tiles, takes 373 us in bfloat16 (0.83 PFLOP/s).
 #include "vt_mx.h"
 #include <type_traits>
 

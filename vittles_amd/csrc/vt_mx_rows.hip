@@ -3,10 +3,14 @@
 // One pass: a team of threads holds the codes of R rows in registers from the dot to the column sums, 16 columns
 // ("a piece": half a block, 16 bytes of E4M3 or 8 of E2M1) a thread and round, and their sums of the columns for the
 // whole kernel.  Partial sums are combined in a fixed order (no atomics: the same bits every time).
-// Bound: HBM for E4M3 (reads alone: 5.4 - 5.9 TB/s), the VALU for E2M1.  An element costs half a conversion to float and
-// one to double, once if its double is kept and twice if not, and two fp64 FMAs: 3.5 to 5 instructions of 4 cycles for 64
-// elements, and about 100 more a round for the sums.  Measured, HVP in TB/s of stored bytes: E4M3 N = 4 10^6, D = 100 4.6;
-// N = 10^5, D = 8192 4.6, D = 20 000 4.4 (474 us); E2M1 3.1, 2.8, 2.7 (391 us); A v 5.9 and 4.2 at most.
+// What bounds it: HBM for E4M3 (A v and A^T u 4.9 to 5.8 TB/s, HVP 4.0 to 4.5; a copy reaches 4.9).  For E2M1 a round's
+// chain -- decode, dots, sums over the waves, barrier, link, columns -- which the one or two workgroups of a CU hardly
+// overlap.  An element costs half a conversion to float and one to double, once if its double is kept and twice if not, and
+// two fp64 FMAs: 3.5 to 5 instructions of 4 cycles for 64 elements, and about 130 more a wave and round for sums, link and
+// addresses.  Of the cycles held the VALU issues in 45 % (gradient, E4M3, N = 10^6, D = 100), 42 % (gradient, E2M1, 20011 x
+// 5003: three of eight waves have no piece there and decode the last one again, all eight evaluate the link) and 74 % (HVP,
+// E4M3, 10^5 x 20 000, which decodes twice).  Medians, HVP in TB/s of stored bytes: E4M3 N = 4 10^6, D = 100 4.5; N = 10^5,
+// D = 8192 4.5, D = 20 000 4.0 - 4.2 (494 - 515 us); E2M1 2.9, 2.7, 2.6 (411 - 419 us).
 // (One wave a round for the gradient's coefficients, handed on through LDS and a second barrier: 5 to 12 % longer.)
 #include "vt_mx.h"
 #include <type_traits>
@@ -455,6 +459,9 @@ __global__ __launch_bounds__(TEAM ? TEAM : 512, TEAM ? 2 : few_waves(OP)) void k
 
 // ---- two passes: rows too wide for one workgroup's registers and LDS ----------------------------------------------------
 // One wave per row takes the dots and leaves t_n in the workspace; then every thread owns eight columns and walks a slab.
+// The dots are far from their bytes: eight bytes of codes a load, v from L2 for every row, a row a wave, nothing fetched
+// ahead.  At 50 000 x 20 353 HVP 1.30 ms (E4M3; E2M1 1.23), gradient 2.03, link 1.71, A v 0.98, A^T u 0.32, where one pass
+// takes 0.50, 0.54, 0.46, 0.37 and 0.36 for twice the numbers (10^5 x 20 000).
 
 // Eight values of a row, columns 8 g .. 8 g + 7.
 template <int FMT>
@@ -559,8 +566,8 @@ struct RowsPlan {
 };
 
 // Rows a round.  One piece a thread: 4, kept as doubles (128 registers).  Two pieces: 4, decoded twice (N = 50 000,
-// D = 16 384: 206 us; 2 kept rows 222).  Three pieces: 4 fit for E2M1; for E4M3 2 (N = 100 000, D = 20 000: 474 us; 4 spill:
-// 985).  Of one piece, two rows a round with more waves resident: 20 to 40 % longer; a round's time is what the VALU issues.
+// D = 16 384: 206 us; 2 kept rows 222).  Three pieces: 4 fit for E2M1; for E4M3 2 (N = 100 000, D = 20 000: about 490 us; 4
+// spill: 985).  Of one piece, two rows a round with more waves resident: 20 to 40 % longer; a round's time is what the VALU issues.
 constexpr int wave_rows(int lanes) { return lanes < 4 ? lanes : 4; }
 constexpr int wide_rows(int cpt, int format) { return cpt == 3 && format == VT_MX_FP8 ? 2 : 4; }
 

@@ -97,8 +97,8 @@ class WeightedGLMObjective(RegisteredObjective):
 
     ``dtype="mxfp8"`` / ``"mxfp4"``, or ``X`` given as ``compact.CompactRows``: COMPACT storage, 8 or 4 bits a feature
     with a scale for every 32 of them.  All row operators (link, gradient, value, HVP and the CG route, A v, A^T u) read
-    the compact rows, at any D, with every vector and sum in double; they compute the objective OF THE STORED values
-    exactly.  There is no Hessian route: ``solver_lib.get_cg_solver`` on ``cg.GLMHessianVectorProduct`` solves."""
+    the compact rows, at any D up to 2^30 (past 20352 in two passes, several times slower), with every vector and sum in
+    double; they compute the objective OF THE STORED values exactly.  There is no Hessian route: ``solver_lib.get_cg_solver`` on ``cg.GLMHessianVectorProduct`` solves."""
 
     def __init__(self, X, y, family="logistic", prior=None, scale=1.0, offset=None,
                  device=None, process_group=None, dtype=torch.float64):
