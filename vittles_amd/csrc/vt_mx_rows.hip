@@ -567,7 +567,8 @@ struct RowsPlan {
 
 // Rows a round.  One piece a thread: 4, kept as doubles (128 registers).  Two pieces: 4, decoded twice (N = 50 000,
 // D = 16 384: 206 us; 2 kept rows 222).  Three pieces: 4 fit for E2M1; for E4M3 2 (N = 100 000, D = 20 000: about 490 us; 4
-// spill: 985).  Of one piece, two rows a round with more waves resident: 20 to 40 % longer; a round's time is what the VALU issues.
+// spill: 985).  Of one piece, two rows a round with more waves resident: 20 to 40 % longer, the sums, the barrier and the link
+// are paid once a round.
 constexpr int wave_rows(int lanes) { return lanes < 4 ? lanes : 4; }
 constexpr int wide_rows(int cpt, int format) { return cpt == 3 && format == VT_MX_FP8 ? 2 : 4; }
 
